@@ -165,6 +165,121 @@ EXPERT_CACHE_API int expert_cache_pregate(const void* x, int T, int ldx, int H,
                                           const void* gate_w, int E, int k, int* out_ids,
                                           cudaStream_t stream);
 
+/* Limits of the layer's arithmetic below: experts per token, hidden and expert width, rank. */
+#define EXPERT_CACHE_EXPERTS_MAX_TOPK 32
+#define EXPERT_CACHE_EXPERTS_MAX_DIM 32768
+#define EXPERT_CACHE_LORA_MAX_RANK 256
+
+/* The router: the k best experts of each token and their weights.
+ *
+ * The score of an expert is the dot product of x[t, :H] (bf16, row stride ldx elements)
+ * with gate_w[e, :H] (bf16, [E, H] row-major), summed in 64 bits, so that the choice does
+ * not depend on the order of a sum.
+ *   scoring 0  softmax over all E experts; the k largest scores are picked
+ *   scoring 1  sigmoid of each score; the k largest sigmoid + bias[e] are picked (bias:
+ *              fp32 [E] or NULL), the weight is the sigmoid alone
+ *   renormalize != 0 divides a token's weights by their sum; then all are multiplied by
+ *   `scale`.
+ * out_ids [T*k] int32 and out_weights [T*k] fp32 are in descending order of the picked
+ * value.  Ties go to the lower expert id.  NaN and -inf are never picked: where fewer than
+ * k experts are left, the id is -1 and the weight 0.
+ *
+ * Returns -1 if:
+ *   - T < 0;
+ *   - H <= 0, H % 8 != 0 or H > EXPERT_CACHE_PREGATE_MAX_HIDDEN;
+ *   - ldx < H or ldx % 8 != 0;
+ *   - E <= 0 or E > EXPERT_CACHE_PREGATE_MAX_EXPERTS;
+ *   - k outside [1, min(E, EXPERT_CACHE_EXPERTS_MAX_TOPK)];
+ *   - scoring outside {0, 1}, or a bias with scoring 0;
+ *   - x or gate_w is not 16-byte aligned.
+ * T == 0 enqueues nothing.
+ *
+ * Has no counterpart in the reference, whose routing is vLLM's. */
+EXPERT_CACHE_API int expert_cache_route(const void* x, int T, int ldx, int H,
+                                        const void* gate_w, int E, int k, int scoring,
+                                        int renormalize, const float* bias, float scale,
+                                        float* out_weights, int* out_ids,
+                                        cudaStream_t stream);
+
+/* Weight types of expert_cache_experts. */
+#define EXPERT_CACHE_BF16 0
+#define EXPERT_CACHE_INT8 1
+#define EXPERT_CACHE_FP8 2 /* e4m3 */
+
+/* Bytes of device workspace that expert_cache_experts (r = 0) or expert_cache_experts_lora
+ * needs for these sizes.  Returns -1 on their rules for the sizes. */
+EXPERT_CACHE_API int expert_cache_experts_workspace(int T, int k, int H, int I, int wtype,
+                                                    int r, long* bytes);
+
+/* The experts of an MoE layer for a few tokens, read from the cache's slots:
+ *
+ *   out[t] = sum_j weights[t, j] * W2[s] (silu(G) * U),  [G; U] = W13[s] x[t]
+ *
+ * with s = ids[t, j], or expert_map[ids[t, j]] where a map is given (the cache's `table`
+ * with expert ids, or the composed map of expert_cache_manage_ep with global ids).  A pair
+ * whose id or slot is out of range adds nothing; its weight is not read into the result.
+ * A token without any pair gets zeros.  The same slot may appear more than once in a token.
+ *
+ *   x        [T, H] bf16, row stride ldx elements         out  [T, H] bf16, stride ldo
+ *   ids      [T, k] int32                                 weights [T, k] fp32
+ *   w13      [S, 2I, H] (gate rows, then up rows)         w2   [S, H, I]
+ *   wtype    EXPERT_CACHE_BF16, or EXPERT_CACHE_INT8 / EXPERT_CACHE_FP8 with
+ *            w13_scale [S, 2I] and w2_scale [S, H] fp32 (one per output row; NULL for
+ *            bf16).  x and h are then quantised per row: q = round(v * Q / m), scale m / Q,
+ *            m = max|v| (at least 1e-10), Q = 127 or 448.
+ *
+ * Sums are in fp32 (int32 for int8 products); h is not rounded to 16 bits.  The result does
+ * not depend on T or on other tokens, up to the order of the sum over a token's experts
+ * (ascending slot).  No atomics: the same inputs give the same bits.
+ *
+ * The weights are read once per 32 tokens (fewer where the tables or 8-bit rows of x do
+ * not fit on chip): meant for the steps a cache serves, tokens * k <= S.
+ *
+ * `workspace` (256-byte aligned) is the call's own from its start to its end on `stream`;
+ * nothing is kept in it between calls.  out must not overlap an input.
+ *
+ * Returns -1 if:
+ *   - T < 0, k outside [1, EXPERT_CACHE_EXPERTS_MAX_TOPK], S outside
+ *     [1, EXPERT_CACHE_MAX_SLOTS], an expert_map with n_map <= 0, wtype unknown;
+ *   - H or I outside [1, EXPERT_CACHE_EXPERTS_MAX_DIM] or not a multiple of 8 (16 for 8-bit
+ *     weights);
+ *   - ldx < H, ldx % 8 != 0 or ldo < H;
+ *   - a needed pointer is NULL, scales are given for bf16 or missing otherwise, or x, w13 or
+ *     w2 is not 16-byte aligned;
+ *   - the workspace is too small or misaligned.
+ * T == 0 enqueues nothing.
+ *
+ * Has no counterpart in the reference, which leaves the layer to vLLM's kernels. */
+EXPERT_CACHE_API int expert_cache_experts(
+    const void* x, int T, int ldx, int H, const int* ids, const float* weights, int k,
+    const int* expert_map, int n_map, const void* w13, const float* w13_scale, const void* w2,
+    const float* w2_scale, int wtype, int S, int I, void* out, int ldo, void* workspace,
+    long workspace_bytes, cudaStream_t stream);
+
+/* expert_cache_experts with low-rank adapters of many requests at once beside the experts'
+ * shared projections.  Token t of adapter a = adapter[t] (outside [0, L): none) adds, for
+ * each of its experts e = ids[t, j] (the id before expert_map; outside [0, E): none),
+ *
+ *   scaling[a] * B13[a, e] (A13[a, e] x[t])  to [G; U]  (the first r rows of A13 and the
+ *                                            first I rows of B13 are the gate's)
+ *   scaling[a] * B2[a, e] (A2[a, e] h)       to the expert's output
+ *
+ * from the unquantised x and h.  Adapters are indexed by expert, not by slot: they need not
+ * move when the cache moves an expert.
+ *
+ *   a13 [L, E, 2r, H]   b13 [L, E, 2I, r]   a2 [L, E, r, I]   b2 [L, E, H, r]   (bf16)
+ *   adapter [T] int32   scaling [L] fp32
+ *
+ * Returns -1 on expert_cache_experts' rules, when L or E <= 0, when r is not a multiple of
+ * 8 in [8, EXPERT_CACHE_LORA_MAX_RANK], or when a pointer is NULL or an adapter matrix is
+ * not 16-byte aligned. */
+EXPERT_CACHE_API int expert_cache_experts_lora(
+    const void* x, int T, int ldx, int H, const int* ids, const float* weights, int k,
+    const int* expert_map, int n_map, const void* w13, const float* w13_scale, const void* w2,
+    const float* w2_scale, int wtype, int S, int I, const int* adapter, const void* a13,
+    const void* b13, const void* a2, const void* b2, const float* scaling, int L, int E, int r,
+    void* out, int ldo, void* workspace, long workspace_bytes, cudaStream_t stream);
+
 /* Largest expert count of expert_cache_fused (reference expert_cache.hip:341, MAXE). */
 #define EXPERT_CACHE_FUSED_MAX_EXPERTS 1024
 

@@ -17,7 +17,8 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SRC = HERE / "csrc" / "expert_cache.cu"
+SRC = HERE / "csrc" / "expert_cache.cu"        # the cache: policy step, copies
+SOURCES = [SRC, HERE / "csrc" / "moe.cu"]      # and the layer's arithmetic
 HEADER = ROOT / "include" / "expert_cache.h"
 OUT = HERE / "vllm_expert_cache" / "libexpertcache.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -32,11 +33,11 @@ def exported_symbols(path: Path = HEADER) -> list[str]:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    deps = [SRC, HEADER]
+    deps = [*SOURCES, HEADER]
     if (OUT.exists() and not force
             and OUT.stat().st_mtime >= max(p.stat().st_mtime for p in deps)):
         return OUT
-    cmd = [NVCC, *FLAGS, "-I", str(ROOT / "include"), str(SRC), "-o", str(OUT)]
+    cmd = [NVCC, *FLAGS, "-I", str(ROOT / "include"), *map(str, SOURCES), "-o", str(OUT)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     subprocess.run(cmd, check=True)

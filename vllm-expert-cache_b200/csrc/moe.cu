@@ -1,0 +1,1098 @@
+// The cached MoE layer's arithmetic for B200 (sm_100a): the experts of a few tokens read
+// from the cache's slots (expert_cache_experts), the same with low-rank adapters of many
+// requests (expert_cache_experts_lora), and the router that feeds them
+// (expert_cache_route).
+//
+//   out[t] = sum_j w[t,j] * W2[s] h,   h = silu(G) * U,   [G; U] = W13[s] x[t],
+//   s = the slot of the token's j-th expert.
+//
+// Each routed expert's weights are read once, 3*H*I elements for a handful of tokens: the
+// layer is bound by those bytes, so everything else is arranged around streaming them.
+//
+//   up_kernel     [G; U] and h.  The routed slots' rows are one flat range, split evenly
+//                 over the CTAs.  A tile is 8 (gate, up) row pairs: as the 16 rows of an
+//                 m16n8k16 product they leave gate and up of a token in one thread.  The
+//                 tokens are the 8 columns, so one read of a weight serves them all.
+//   mid_kernel    8-bit weights only: quantises h per (token, expert) row, which needs the
+//                 row's maximum; with adapters: A2 h.
+//   down_kernel   a CTA owns a few rows of `out` and runs over all routed slots, so the
+//                 sum over a token's experts stays in its registers: no atomics, no second
+//                 pass, the same order of sums in every run.
+//
+// tcgen05 is not used: at n tokens an expert the layer does 2n flops a weight, far below
+// the ridge for the token counts a cached step has, and mma.sync takes the weights from
+// registers in the order they arrive.
+//
+// Precision: sums in fp32 (int32 for int8, exact).  h keeps 16 bits of mantissa as the sum
+// of two bf16 values (hi + lo), two products with the same weights, so that the layer
+// rounds once, at its output; 8-bit layers round x and h as their scheme defines.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <climits>
+#include <cstdint>
+
+#include "expert_cache.h"
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxPairs = EXPERT_CACHE_MAX_SLOTS;   // (token, expert) pairs of one launch
+constexpr int kMaxTokens = 32;                      // tokens of one launch (4 column tiles)
+constexpr int kMaxCols = 16384;                     // pairs x padded tokens of one launch
+constexpr int kStageBytes = 112 * 1024;             // largest staged x
+
+enum WType { kBf16 = 0, kInt8 = 1, kFp8 = 2 };
+
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void release_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+struct Adapters {
+  const int* index;                // [T] adapter of each token, outside [0, L) = none
+  const __nv_bfloat16 *a13, *b13, *a2, *b2;
+  const float* scaling;            // [L]
+  int L, E, r;                     // r = 0: no adapters
+};
+
+struct ExpertsArgs {
+  const __nv_bfloat16* x;
+  const int* ids;
+  const float* weights;
+  const int* map;                  // nullptr: ids are slots
+  const uint8_t *w13, *w2;
+  const float *s13, *s2;
+  __nv_bfloat16* out;
+  long long ldx, ldo;
+  int T, k, H, I, S, n_map;
+  // workspace
+  __nv_bfloat16 *h_hi, *h_lo;      // bf16 weights: weights[t,j] * h in two parts [P][I]
+  float* h;                        // 8-bit weights: h [P][I]
+  uint8_t* hq;                     // 8-bit weights: quantised h [P][I]
+  float* h_scale;                  // 8-bit weights: its scale x weights[t,j] [P]
+  float *u, *v;                    // adapters: c A13 x [P][2r], c w A2 h [P][r]
+  Adapters lora;
+};
+
+// ---------------------------------------------------------------------------------------
+// Which pairs go to which slot.  An entry is one routed slot; its columns are the tokens,
+// each with the pair that brought it there or none.  A token that names a slot twice gets
+// an entry of its own for every repetition, so that a column never holds two pairs.
+
+struct Routing {
+  int* entries;          // [1]
+  unsigned* bits;        // [kMaxPairs / 32] routed slots
+  int* base;             // [kMaxPairs / 32] entries before a word of `bits`
+  short* slot;           // [P] slot of an entry
+  short* pair_slot;      // [P] slot of a pair, -1 = none
+  unsigned char* mask;   // [P] column tiles of an entry with a pair in them
+  short* col;            // [P][8 NT] pair of an entry's column, -1 = none
+};
+
+constexpr int kRoutingFixed = 16 + (kMaxPairs / 32) * 8;
+
+__host__ __device__ inline size_t routing_bytes(int P, int NT) {
+  return kRoutingFixed + ((size_t)P * (2 + 2 + 1 + 16 * NT) + 15) / 16 * 16;
+}
+
+__device__ __forceinline__ Routing routing_at(unsigned char* base, int P, int NT) {
+  Routing r;
+  r.entries = reinterpret_cast<int*>(base);
+  r.bits = reinterpret_cast<unsigned*>(base + 16);
+  r.base = reinterpret_cast<int*>(r.bits + kMaxPairs / 32);
+  r.col = reinterpret_cast<short*>(base + kRoutingFixed);
+  r.slot = r.col + (size_t)P * 8 * NT;
+  r.pair_slot = r.slot + P;
+  r.mask = reinterpret_cast<unsigned char*>(r.pair_slot + P);
+  return r;
+}
+
+__device__ __forceinline__ int slot_of(const ExpertsArgs& a, int p) {
+  int s = a.ids[p];
+  if (a.map) s = (s >= 0 && s < a.n_map) ? a.map[s] : -1;
+  return (s >= 0 && s < a.S) ? s : -1;
+}
+
+// Whole CTA; ends with a barrier.  Entries are in ascending slot order (repetitions after
+// them in pair order), so sums over entries have one order.
+template <int NT>
+__device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
+  const int P = a.T * a.k, tid = threadIdx.x;
+  constexpr int kWords = kMaxPairs / 32;
+  if (tid < kWords) r.bits[tid] = 0;
+  if (tid == 0) r.entries[1] = 0;       // set when some token repeats a slot
+  for (int i = tid; i < P * 8 * NT / 2; i += kThreads)
+    reinterpret_cast<int*>(r.col)[i] = -1;
+  for (int p = tid; p < P; p += kThreads) {
+    r.pair_slot[p] = (short)slot_of(a, p);
+    r.mask[p] = 0;
+  }
+  __syncthreads();
+  bool again = false;
+  for (int p = tid; p < P; p += kThreads) {
+    const int s = r.pair_slot[p];
+    if (s < 0) continue;
+    for (int q = p - p % a.k; q < p; ++q) again |= r.pair_slot[q] == s;
+    atomicOr(&r.bits[s >> 5], 1u << (s & 31));
+  }
+  if (again) r.entries[1] = 1;
+  __syncthreads();
+  if (tid < 32) {
+    const int n = __popc(r.bits[tid]);
+    int sum = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, off);
+      if (tid >= off) sum += o;
+    }
+    r.base[tid] = sum - n;
+    if (tid == 31) r.entries[0] = sum;
+  }
+  __syncthreads();
+  const bool repeats = r.entries[1] != 0;
+  for (int p = tid; p < P; p += kThreads) {
+    const int s = r.pair_slot[p];
+    if (s < 0) continue;
+    bool first = true;
+    if (repeats)
+      for (int q = p - p % a.k; q < p; ++q) first &= r.pair_slot[q] != s;
+    if (!first) continue;
+    const int e = r.base[s >> 5] + __popc(r.bits[s >> 5] & ((1u << (s & 31)) - 1u));
+    const int t = p / a.k;
+    r.slot[e] = (short)s;
+    r.col[(size_t)e * 8 * NT + t] = (short)p;
+  }
+  __syncthreads();
+  if (repeats && tid == 0) {
+    int n = r.entries[0];
+    for (int p = 0; p < P; ++p) {
+      const int s = r.pair_slot[p];
+      bool first = true;
+      for (int q = p - p % a.k; q < p; ++q) first &= r.pair_slot[q] != s;
+      if (s < 0 || first) continue;
+      r.slot[n] = (short)s;
+      r.col[(size_t)n * 8 * NT + p / a.k] = (short)p;
+      ++n;
+    }
+    r.entries[0] = n;
+  }
+  if (repeats) __syncthreads();
+  const int D = r.entries[0];
+  for (int i = tid; i < D * NT; i += kThreads) {
+    const int e = i / NT, nt = i - e * NT;
+    const uint4 c = reinterpret_cast<const uint4*>(r.col)[i];
+    const bool any = (c.x & c.y & c.z & c.w) != 0xffffffffu;
+    if (NT == 1) r.mask[e] = any;
+    else if (any) atomicOr(reinterpret_cast<unsigned*>(r.mask) + (e >> 2), 1u << (8 * (e & 3) + nt));
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------
+// One chunk: 64 bytes of each of 16 weight rows.  Lane (g = lane / 4, q = lane % 4) holds 16
+// bytes of rows g and g + 8 and, of column g, the same 16 bytes: which of the chunk's
+// columns an index of the product stands for is free as long as both operands agree, so
+// every lane loads whole 16-byte vectors.
+
+template <int WT>
+struct Kind {
+  static constexpr int kItem = WT == kBf16 ? 2 : 1;      // bytes per weight
+  static constexpr int kVec = 16 / kItem;                // weights per 16 bytes
+  static constexpr int kChunk = 4 * kVec;                // columns per chunk
+  using Acc = float;
+};
+template <>
+struct Kind<kInt8> {
+  static constexpr int kItem = 1, kVec = 16, kChunk = 64;
+  using Acc = int;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2,
+                                         unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2,
+                                        unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2,
+                                       unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two e4m3 values (the low 16 bits) as two fp16 values, exactly.
+__device__ __forceinline__ unsigned e4m3x2_to_f16x2(unsigned v) {
+  unsigned r;
+  asm("{.reg .b16 t, u; mov.b32 {t, u}, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// acc += (16 rows: a, b) x (8 columns: v) over one chunk.
+__device__ __forceinline__ void chunk_mma_bf16(float (&c)[4], const uint4& a, const uint4& b,
+                                               const uint4& v) {
+  mma_bf16(c, a.x, b.x, a.y, b.y, v.x, v.y);
+  mma_bf16(c, a.z, b.z, a.w, b.w, v.z, v.w);
+}
+__device__ __forceinline__ void chunk_mma_s8(int (&c)[4], const uint4& a, const uint4& b,
+                                             const uint4& v) {
+  mma_s8(c, a.x, b.x, a.y, b.y, v.x, v.y);
+  mma_s8(c, a.z, b.z, a.w, b.w, v.z, v.w);
+}
+
+// 16 e4m3 values as fp16: lane's words for four m16n8k16 products.
+struct Wide {
+  unsigned lo[4], hi[4];
+};
+__device__ __forceinline__ Wide widen(const uint4& v) {
+  Wide w;
+  const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w.lo[i] = e4m3x2_to_f16x2(u[i]);
+    w.hi[i] = e4m3x2_to_f16x2(u[i] >> 16);
+  }
+  return w;
+}
+__device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, const Wide& b,
+                                              const uint4& v) {
+  const Wide w = widen(v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mma_f16(c, a.lo[i], b.lo[i], a.hi[i], b.hi[i], w.lo[i], w.hi[i]);
+}
+
+__device__ __forceinline__ uint4 load_weights(const uint8_t* p) {
+  uint4 r;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+      : "l"(p));
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------
+// Quantised rows: q = round(v * Q / max|v|), scale = max|v| / Q.  The product v * Q of a
+// bf16 v is exact in fp32 and the division is correctly rounded, so a quotient that lies on
+// the border between two values is seen as such.
+
+template <int WT>
+__device__ __forceinline__ unsigned quantise(float v, float top) {
+  if (WT == kInt8) return (unsigned)(unsigned char)(signed char)__float2int_rn(v * 127.f / top);
+  return __nv_cvt_float_to_fp8(v * 448.f / top, __NV_SATFINITE, __NV_E4M3);
+}
+template <int WT>
+__device__ __forceinline__ float quant_scale(float top) {
+  return top / (WT == kInt8 ? 127.f : 448.f);
+}
+
+// max |v| that keeps a NaN (fmaxf would drop it).
+__device__ __forceinline__ float max_abs(float m, float v) {
+  v = fabsf(v);
+  return (v > m || v != v) ? v : m;
+}
+__device__ __forceinline__ float warp_max_abs(float m) {
+#pragma unroll
+  for (int off = 16; off; off >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, off));
+  return m;
+}
+__device__ __forceinline__ float clamp_top(float m) { return m < 1e-10f ? 1e-10f : m; }
+
+// x of the CTA's tokens in shared memory as [chunk][T][64 bytes] (zeros past H), quantised
+// for 8-bit weights with the scales in `xs`.  A warp takes a token.  No barrier.
+template <int WT>
+__device__ void stage_x(const ExpertsArgs& a, unsigned char* st, float* xs) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kChunk = Kind<WT>::kChunk, kVec = Kind<WT>::kVec;
+  const int C = (a.H + kChunk - 1) / kChunk;
+  for (int t = warp; t < a.T; t += kWarps) {
+    const __nv_bfloat16* x = a.x + t * a.ldx;
+    float top = 0.f;
+    if (WT != kBf16) {
+      for (int i = lane * 8; i < a.H; i += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + i);
+        const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          top = max_abs(top, __uint_as_float(u[j] << 16));
+          top = max_abs(top, __uint_as_float(u[j] & 0xffff0000u));
+        }
+      }
+      top = clamp_top(warp_max_abs(top));
+      if (lane == 0) xs[t] = quant_scale<WT>(top);
+    }
+    for (int i = lane; i < C * 4; i += 32) {       // 16-byte pieces
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (i * kVec < a.H) {
+        const uint4* src = reinterpret_cast<const uint4*>(x + i * kVec);
+        if (WT == kBf16) {
+          o = src[0];
+        } else {
+          unsigned w[4];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4 v = src[half];
+            const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              w[2 * half + j] =
+                  quantise<WT>(__uint_as_float(u[2 * j] << 16), top) |
+                  quantise<WT>(__uint_as_float(u[2 * j] & 0xffff0000u), top) << 8 |
+                  quantise<WT>(__uint_as_float(u[2 * j + 1] << 16), top) << 16 |
+                  quantise<WT>(__uint_as_float(u[2 * j + 1] & 0xffff0000u), top) << 24;
+          }
+          o = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      *reinterpret_cast<uint4*>(st + ((size_t)(i >> 2) * a.T + t) * 64 + (i & 3) * 16) = o;
+    }
+  }
+}
+
+// The adapter of a pair, or -1; *matrix = its index among the [L][E] adapter matrices.
+__device__ __forceinline__ int adapter_of(const ExpertsArgs& a, int p, long long* matrix) {
+  const int t = p / a.k, l = a.lora.index[t], e = a.ids[p];
+  if (l < 0 || l >= a.lora.L || e < 0 || e >= a.lora.E) return -1;
+  *matrix = (long long)l * a.lora.E + e;
+  return l;
+}
+
+// sum_j b[j] * u[j], r a multiple of 8, b 16-byte aligned bf16, u fp32.
+__device__ __forceinline__ float dot_row(const __nv_bfloat16* b, const float* u, int r) {
+  float s = 0.f;
+  for (int j = 0; j < r; j += 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(b + j);
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s += __uint_as_float(w[i] << 16) * u[j + 2 * i];
+      s += __uint_as_float(w[i] & 0xffff0000u) * u[j + 2 * i + 1];
+    }
+  }
+  return s;
+}
+
+// ---------------------------------------------------------------------------------------
+// u[p] = c A13[adapter, expert] x[t]: one warp per row of A13.
+
+__global__ void __launch_bounds__(kThreads) shrink_kernel(const __grid_constant__ ExpertsArgs a) {
+  grid_dependency_wait();
+  release_dependents();
+  const int p = blockIdx.x, lane = threadIdx.x & 31;
+  const int row = blockIdx.y * kWarps + (threadIdx.x >> 5);
+  const int rows = 2 * a.lora.r;
+  long long m;
+  if (row >= rows || slot_of(a, p) < 0) return;
+  const int l = adapter_of(a, p, &m);
+  if (l < 0) return;
+  const __nv_bfloat16* w = a.lora.a13 + (m * rows + row) * a.H;
+  const __nv_bfloat16* x = a.x + (p / a.k) * a.ldx;
+  float s = 0.f;
+  for (int i = lane * 8; i < a.H; i += 256) {
+    const uint4 wv = *reinterpret_cast<const uint4*>(w + i);
+    const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
+    const unsigned ww[4] = {wv.x, wv.y, wv.z, wv.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s += __uint_as_float(ww[j] << 16) * __uint_as_float(xw[j] << 16);
+      s += __uint_as_float(ww[j] & 0xffff0000u) * __uint_as_float(xw[j] & 0xffff0000u);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  if (lane == 0) a.u[(size_t)p * rows + row] = s * a.lora.scaling[l];
+}
+
+// ---------------------------------------------------------------------------------------
+// up
+
+template <int NT>
+constexpr int kRed = kWarps * 16 * 8 * NT;   // values in one buffer of the warps' partial sums
+
+template <int WT, int NT>
+__global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__ ExpertsArgs a,
+                                                         int staged) {
+  using K = Kind<WT>;
+  using Acc = typename K::Acc;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int P = a.T * a.k;
+  const Routing rt = routing_at(smem, P, NT);
+  Acc* red = reinterpret_cast<Acc*>(smem + routing_bytes(P, NT));
+  float* xs = reinterpret_cast<float*>(red + 2 * kRed<NT>);
+  unsigned char* st = reinterpret_cast<unsigned char*>(xs + kMaxTokens);
+
+  grid_dependency_wait();
+  release_dependents();
+  build_routing<NT>(a, rt);
+  const int D = rt.entries[0];
+  const long long R = (long long)D * a.I;
+  const int r0 = (int)(R * blockIdx.x / gridDim.x), r1 = (int)(R * (blockIdx.x + 1) / gridDim.x);
+  if (r0 >= r1) return;
+  if (staged) {
+    stage_x<WT>(a, st, xs);
+    __syncthreads();
+  }
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int C = (a.H + K::kChunk - 1) / K::kChunk;
+  const long long row_bytes = (long long)a.H * K::kItem;
+  int buf = 0;
+  for (int row = r0, n; row < r1; row += n, buf ^= 1) {
+    const int e = row / a.I, i0 = row - e * a.I;
+    n = min(8, min(r1 - row, a.I - i0));
+    const int slot = rt.slot[e];
+    const unsigned mask = rt.mask[e];
+    const uint8_t* w = a.w13 + ((long long)slot * 2 * a.I + i0 + g) * row_bytes + q * 16;
+    Acc acc[NT][4] = {};
+    for (int c = warp; c < C; c += kWarps) {
+      uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
+      const bool in = c * K::kChunk + q * K::kVec < a.H;
+      if (g < n && in) {
+        wa = load_weights(w + c * 64);
+        wb = load_weights(w + a.I * row_bytes + c * 64);
+      }
+      Wide fa, fb;
+      if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (NT > 1 && !(mask >> nt & 1)) continue;
+        const int t = nt * 8 + g;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (t < a.T) {
+          if (staged)
+            v = *reinterpret_cast<const uint4*>(st + ((size_t)c * a.T + t) * 64 + q * 16);
+          else if (in)
+            v = *reinterpret_cast<const uint4*>(a.x + t * a.ldx + c * K::kChunk + q * K::kVec);
+        }
+        if constexpr (WT == kBf16) chunk_mma_bf16(acc[nt], wa, wb, v);
+        if constexpr (WT == kInt8) chunk_mma_s8(acc[nt], wa, wb, v);
+        if constexpr (WT == kFp8) chunk_mma_fp8(acc[nt], fa, fb, v);
+      }
+    }
+    // partial sums of the warps: [warp][row][column]
+    Acc* mine = red + buf * kRed<NT> + warp * 16 * 8 * NT;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = nt * 8 + 2 * q;
+      mine[g * 8 * NT + c] = acc[nt][0];
+      mine[g * 8 * NT + c + 1] = acc[nt][1];
+      mine[(g + 8) * 8 * NT + c] = acc[nt][2];
+      mine[(g + 8) * 8 * NT + c + 1] = acc[nt][3];
+    }
+    __syncthreads();
+    for (int o = tid; o < 8 * a.T; o += kThreads) {
+      const int i = o & 7, t = o >> 3;
+      const int p = rt.col[(size_t)e * 8 * NT + t];
+      if (i >= n || p < 0) continue;
+      const Acc* src = red + buf * kRed<NT> + i * 8 * NT + t;
+      Acc sg = 0, su = 0;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        sg += src[k * 16 * 8 * NT];
+        su += src[(k * 16 + 8) * 8 * NT];
+      }
+      float gate = (float)sg, up = (float)su;
+      const int r = i0 + i;
+      if (WT != kBf16) {
+        gate *= xs[t] * a.s13[(long long)slot * 2 * a.I + r];
+        up *= xs[t] * a.s13[(long long)slot * 2 * a.I + a.I + r];
+      }
+      long long m;
+      if (a.lora.r && adapter_of(a, p, &m) >= 0) {
+        const __nv_bfloat16* b = a.lora.b13 + (m * 2 * a.I + r) * a.lora.r;
+        const float* u = a.u + (size_t)p * 2 * a.lora.r;
+        gate += dot_row(b, u, a.lora.r);
+        up += dot_row(b + (long long)a.I * a.lora.r, u + a.lora.r, a.lora.r);
+      }
+      float h = gate / (1.f + expf(-gate)) * up;
+      if (WT == kBf16) {
+        h *= a.weights[p];
+        const __nv_bfloat16 hi = __float2bfloat16(h);
+        const float back = __bfloat162float(hi);
+        // (an infinite hi has no remainder)
+        const __nv_bfloat16 lo = __float2bfloat16(isfinite(back) ? h - back : 0.f);
+        a.h_hi[(size_t)p * a.I + r] = hi;
+        a.h_lo[(size_t)p * a.I + r] = lo;
+      } else {
+        a.h[(size_t)p * a.I + r] = h;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// mid: one CTA per pair
+
+template <int WT>
+__global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ ExpertsArgs a) {
+  grid_dependency_wait();
+  release_dependents();
+  const int p = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (slot_of(a, p) < 0) return;
+  const size_t at = (size_t)p * a.I;
+  if (WT != kBf16) {
+    __shared__ float tops[kWarps];
+    float top = 0.f;
+    for (int i = tid * 4; i < a.I; i += kThreads * 4) {
+      const float4 v = *reinterpret_cast<const float4*>(a.h + at + i);
+      top = max_abs(max_abs(max_abs(max_abs(top, v.x), v.y), v.z), v.w);
+    }
+    top = warp_max_abs(top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = max_abs(top, tops[w]);
+    top = clamp_top(top);
+    if (tid == 0) a.h_scale[p] = quant_scale<WT>(top) * a.weights[p];
+    for (int i = tid * 4; i < a.I; i += kThreads * 4) {
+      const float4 v = *reinterpret_cast<const float4*>(a.h + at + i);
+      *reinterpret_cast<unsigned*>(a.hq + at + i) =
+          quantise<WT>(v.x, top) | quantise<WT>(v.y, top) << 8 | quantise<WT>(v.z, top) << 16 |
+          quantise<WT>(v.w, top) << 24;
+    }
+  }
+  long long m;
+  if (a.lora.r == 0) return;
+  const int l = adapter_of(a, p, &m);
+  if (l < 0) return;
+  for (int row = warp; row < a.lora.r; row += kWarps) {
+    const __nv_bfloat16* w = a.lora.a2 + (m * a.lora.r + row) * a.I;
+    float s = 0.f;
+    for (int i = lane * 8; i < a.I; i += 256) {
+      const uint4 wv = *reinterpret_cast<const uint4*>(w + i);
+      const unsigned ww[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float h = WT == kBf16 ? __bfloat162float(a.h_hi[at + i + j]) +
+                                          __bfloat162float(a.h_lo[at + i + j])
+                                    : a.h[at + i + j];
+        s += __uint_as_float(j & 1 ? ww[j / 2] & 0xffff0000u : ww[j / 2] << 16) * h;
+      }
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    // bf16 weights: h already carries the routing weight
+    if (lane == 0)
+      a.v[(size_t)p * a.lora.r + row] =
+          s * a.lora.scaling[l] * (WT == kBf16 ? 1.f : a.weights[p]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// down
+
+template <int WT, int NT>
+__global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant__ ExpertsArgs a) {
+  using K = Kind<WT>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int P = a.T * a.k;
+  const Routing rt = routing_at(smem, P, NT);
+  float* red = reinterpret_cast<float*>(smem + routing_bytes(P, NT));
+
+  grid_dependency_wait();
+  release_dependents();
+  const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
+  const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x);
+  if (r0 >= r1) return;
+  build_routing<NT>(a, rt);
+  const int D = rt.entries[0];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int C = (a.I + K::kChunk - 1) / K::kChunk;
+  const long long row_bytes = (long long)a.I * K::kItem;
+  for (int row = r0, n; row < r1; row += n) {
+    n = min(16, r1 - row);
+    float acc[NT][4] = {};
+    int e = 0, c = warp;
+    while (true) {
+      while (e < D && c >= C) { c -= C; ++e; }
+      if (e >= D) break;
+      const long long first = (long long)rt.slot[e] * a.H + row;
+      const unsigned mask = rt.mask[e];
+      const bool in = c * K::kChunk + q * K::kVec < a.I;
+      uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
+      if (in && g < n) wa = load_weights(a.w2 + (first + g) * row_bytes + c * 64 + q * 16);
+      if (in && g + 8 < n) wb = load_weights(a.w2 + (first + g + 8) * row_bytes + c * 64 + q * 16);
+      Wide fa, fb;
+      if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
+      float rf0 = 0.f, rf1 = 0.f;
+      if (WT != kBf16) {
+        if (g < n) rf0 = a.s2[first + g];
+        if (g + 8 < n) rf1 = a.s2[first + g + 8];
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (NT > 1 && !(mask >> nt & 1)) continue;
+        const short* col = rt.col + (size_t)e * 8 * NT + nt * 8;
+        const int p = col[g];
+        const long long at = (long long)p * a.I + c * K::kChunk + q * K::kVec;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if constexpr (WT == kBf16) {
+          uint4 v2 = v;
+          if (p >= 0 && in) {
+            v = *reinterpret_cast<const uint4*>(a.h_hi + at);
+            v2 = *reinterpret_cast<const uint4*>(a.h_lo + at);
+          }
+          chunk_mma_bf16(acc[nt], wa, wb, v);
+          chunk_mma_bf16(acc[nt], wa, wb, v2);
+        } else {
+          if (p >= 0 && in) v = *reinterpret_cast<const uint4*>(a.hq + at);
+          const int p0 = col[2 * q], p1 = col[2 * q + 1];
+          const float c0 = p0 >= 0 ? a.h_scale[p0] : 0.f, c1 = p1 >= 0 ? a.h_scale[p1] : 0.f;
+          typename K::Acc part[4] = {};
+          if constexpr (WT == kInt8) chunk_mma_s8(part, wa, wb, v);
+          if constexpr (WT == kFp8) chunk_mma_fp8(part, fa, fb, v);
+          acc[nt][0] += (float)part[0] * (rf0 * c0);
+          acc[nt][1] += (float)part[1] * (rf0 * c1);
+          acc[nt][2] += (float)part[2] * (rf1 * c0);
+          acc[nt][3] += (float)part[3] * (rf1 * c1);
+        }
+      }
+      c += kWarps;
+    }
+    float* mine = red + warp * 16 * 8 * NT;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + 2 * q;
+      mine[g * 8 * NT + col] = acc[nt][0];
+      mine[g * 8 * NT + col + 1] = acc[nt][1];
+      mine[(g + 8) * 8 * NT + col] = acc[nt][2];
+      mine[(g + 8) * 8 * NT + col + 1] = acc[nt][3];
+    }
+    __syncthreads();
+    for (int o = tid; o < 16 * a.T; o += kThreads) {
+      const int i = o & 15, t = o >> 4;
+      if (i >= n) continue;
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) s += red[(k * 16 + i) * 8 * NT + t];
+      if (a.lora.r) {
+        for (int p = t * a.k; p < (t + 1) * a.k; ++p) {
+          long long m;
+          if (rt.pair_slot[p] < 0 || adapter_of(a, p, &m) < 0) continue;
+          s += dot_row(a.lora.b2 + (m * a.H + row + i) * a.lora.r,
+                       a.v + (size_t)p * a.lora.r, a.lora.r);
+        }
+      }
+      a.out[t * a.ldo + row + i] = __float2bfloat16(s);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// route: one CTA per token.  Scores are sums in 64 bits of exact products, so which expert
+// is the k-th best does not hang on the order of a sum.
+
+constexpr int kRouteThreads = 256;
+
+struct RouteArgs {
+  const __nv_bfloat16 *x, *gate;
+  const float* bias;
+  float* weights;
+  int* ids;
+  long long ldx;
+  int T, H, E, k, sigmoid, renorm;
+  float scale;
+};
+
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  double* score = reinterpret_cast<double*>(smem);           // selection key
+  __shared__ double r_val[kRouteThreads / 32];
+  __shared__ int r_idx[kRouteThreads / 32];
+  __shared__ double s_sum, s_max;
+  grid_dependency_wait();
+  release_dependents();
+  const int tok = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int NW = kRouteThreads / 32;
+  const __nv_bfloat16* x = a.x + tok * a.ldx;
+  for (int e = warp; e < a.E; e += NW) {
+    double s = 0.0;
+    for (int i = lane * 8; i < a.H; i += 256) {
+      const uint4 wv = *reinterpret_cast<const uint4*>(a.gate + (long long)e * a.H + i);
+      const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
+      const unsigned ww[4] = {wv.x, wv.y, wv.z, wv.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s += (double)__uint_as_float(ww[j] << 16) * (double)__uint_as_float(xw[j] << 16);
+        s += (double)__uint_as_float(ww[j] & 0xffff0000u) *
+             (double)__uint_as_float(xw[j] & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (lane == 0) {
+      if (a.sigmoid) s = 1.0 / (1.0 + exp(-s)) + (a.bias ? (double)a.bias[e] : 0.0);
+      score[e] = s;
+    }
+  }
+  __syncthreads();
+  if (!a.sigmoid) {
+    double m = -INFINITY;
+    for (int e = tid; e < a.E; e += kRouteThreads) m = fmax(m, score[e]);
+    for (int off = 16; off; off >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if (lane == 0) r_val[warp] = m;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < NW; ++w) m = fmax(m, r_val[w]);
+      s_max = m;
+    }
+    __syncthreads();
+    double sum = 0.0;
+    for (int e = tid; e < a.E; e += kRouteThreads)
+      if (score[e] == score[e]) sum += exp(score[e] - s_max);
+    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) r_val[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < NW; ++w) sum += r_val[w];
+      s_sum = sum;
+    }
+    __syncthreads();
+  }
+  double total = 0.0;
+  double mine = 0.0;       // thread r < k keeps the r-th weight
+  int mine_id = -1;
+  for (int r = 0; r < a.k; ++r) {
+    double bv = -INFINITY;
+    int bi = -1;
+    for (int e = tid; e < a.E; e += kRouteThreads)
+      if (score[e] > bv) { bv = score[e]; bi = e; }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+      const double ov = __shfl_xor_sync(0xffffffffu, bv, off);
+      const int oi = __shfl_xor_sync(0xffffffffu, bi, off);
+      if (oi >= 0 && (bi < 0 || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
+    }
+    if (lane == 0) { r_val[warp] = bv; r_idx[warp] = bi; }
+    __syncthreads();
+    if (tid < 32) {
+      bv = -INFINITY; bi = -1;
+      for (int w = 0; w < NW; ++w)
+        if (r_idx[w] >= 0 && (bi < 0 || r_val[w] > bv || (r_val[w] == bv && r_idx[w] < bi))) {
+          bv = r_val[w];
+          bi = r_idx[w];
+        }
+      double wgt = 0.0;
+      if (bi >= 0) {
+        if (a.sigmoid) wgt = bv - (a.bias ? (double)a.bias[bi] : 0.0);
+        else wgt = exp(bv - s_max) / s_sum;
+      }
+      total += wgt;
+      if (tid == r) { mine = wgt; mine_id = bi; }
+      __syncwarp();
+      if (tid == 0 && bi >= 0) score[bi] = -INFINITY;
+    }
+    __syncthreads();
+  }
+  if (tid < a.k) {
+    if (a.renorm && total > 0.0) mine /= total;
+    a.weights[(long long)tok * a.k + tid] = (float)(mine * (double)a.scale);
+    a.ids[(long long)tok * a.k + tid] = mine_id;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// host side
+
+std::atomic<int> g_sms[kMaxDevices];
+
+int device_sms(int* dev, int* sms) {
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= kMaxDevices)
+    return (int)cudaErrorInvalidDevice;
+  int n = g_sms[d].load(std::memory_order_relaxed);
+  if (n == 0) {
+    const cudaError_t err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d);
+    if (err != cudaSuccess) return (int)err;
+    g_sms[d].store(n, std::memory_order_relaxed);
+  }
+  *dev = d;
+  *sms = n;
+  return 0;
+}
+
+// Raise a kernel's dynamic shared memory limit once per device (`done`: its own flags).
+template <typename Kernel>
+cudaError_t allow_smem(Kernel fn, std::atomic<bool>* done, int dev) {
+  if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  int optin = 0;
+  cudaError_t err = cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (err != cudaSuccess) return err;
+  cudaFuncAttributes fa{};
+  err = cudaFuncGetAttributes(&fa, fn);
+  if (err != cudaSuccess) return err;
+  err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             optin - (int)fa.sharedSizeBytes);
+  if (err == cudaSuccess) done[dev].store(true, std::memory_order_release);
+  return err;
+}
+
+template <typename... Params, typename... Args>
+int launch(void (*fn)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+           const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, fn, Params(args)...);
+}
+
+int chunk_columns(int wtype) { return wtype == kBf16 ? 32 : 64; }
+
+size_t staged_bytes(int T, int H, int wtype) {
+  const int cc = chunk_columns(wtype);
+  return (size_t)((H + cc - 1) / cc) * 64 * T;
+}
+
+int column_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
+
+// Tokens of one launch: as many as fit the column tiles, the pair tables and (8-bit
+// weights, which are multiplied by staged rows only) the shared memory.
+int tokens_per_launch(int T, int k, int H, int wtype) {
+  int n = T < kMaxTokens ? T : kMaxTokens;
+  while (n > 1 && (n * k > kMaxPairs || n * k * 8 * column_tiles(n) > kMaxCols ||
+                   (wtype != kBf16 && staged_bytes(n, H, wtype) > kStageBytes)))
+    --n;
+  return n;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// The workspace's parts for `pairs` pairs; returns its size.
+size_t carve(ExpertsArgs* a, unsigned char* base, size_t pairs, int I, int wtype, int r) {
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    unsigned char* p = base ? base + at : nullptr;
+    at += align256(bytes);
+    return p;
+  };
+  if (wtype == kBf16) {
+    a->h_hi = reinterpret_cast<__nv_bfloat16*>(take(pairs * I * 2));
+    a->h_lo = reinterpret_cast<__nv_bfloat16*>(take(pairs * I * 2));
+  } else {
+    a->h = reinterpret_cast<float*>(take(pairs * I * 4));
+    a->hq = take(pairs * I);
+    a->h_scale = reinterpret_cast<float*>(take(pairs * 4));
+  }
+  if (r) {
+    a->u = reinterpret_cast<float*>(take(pairs * 2 * r * 4));
+    a->v = reinterpret_cast<float*>(take(pairs * r * 4));
+  }
+  return at;
+}
+
+template <int WT, int NT>
+int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
+  static std::atomic<bool> done_up[kMaxDevices], done_down[kMaxDevices];
+  int dev = 0, sms = 0;
+  int rc = device_sms(&dev, &sms);
+  if (rc != 0) return rc;
+  cudaError_t err = allow_smem(up_kernel<WT, NT>, done_up, dev);
+  if (err == cudaSuccess) err = allow_smem(down_kernel<WT, NT>, done_down, dev);
+  if (err != cudaSuccess) return (int)err;
+  const int P = a.T * a.k;
+  if (a.lora.r) {
+    rc = launch(shrink_kernel, dim3(P, (2 * a.lora.r + kWarps - 1) / kWarps), kThreads, 0,
+                stream, a);
+    if (rc != 0) return rc;
+  }
+  const size_t tables = routing_bytes(P, NT), red = (size_t)kRed<NT> * 4;
+  size_t stage = staged_bytes(a.T, a.H, WT);
+  const int staged = stage <= (size_t)kStageBytes;
+  if (!staged) stage = 0;
+  rc = launch(up_kernel<WT, NT>, dim3(sms), kThreads,
+              tables + 2 * red + kMaxTokens * 4 + stage, stream, a, staged);
+  if (rc != 0) return rc;
+  if (WT != kBf16 || a.lora.r) {
+    rc = launch(mid_kernel<WT>, dim3(P), kThreads, 0, stream, a);
+    if (rc != 0) return rc;
+  }
+  return launch(down_kernel<WT, NT>, dim3(sms), kThreads, tables + red, stream, a);
+}
+
+template <int WT>
+int run_type(const ExpertsArgs& a, cudaStream_t stream) {
+  switch (column_tiles(a.T)) {
+    case 1: return run_layer<WT, 1>(a, stream);
+    case 2: return run_layer<WT, 2>(a, stream);
+    default: return run_layer<WT, 4>(a, stream);
+  }
+}
+
+bool misaligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
+
+bool shape_ok(int T, int k, int H, int I, int wtype) {
+  if (T < 0 || k <= 0 || k > EXPERT_CACHE_EXPERTS_MAX_TOPK) return false;
+  if (wtype < kBf16 || wtype > kFp8) return false;
+  const int vec = wtype == kBf16 ? 8 : 16;
+  return H > 0 && H <= EXPERT_CACHE_EXPERTS_MAX_DIM && H % vec == 0 && I > 0 &&
+         I <= EXPERT_CACHE_EXPERTS_MAX_DIM && I % vec == 0;
+}
+
+int experts_checked(ExpertsArgs a, int wtype, void* workspace, long workspace_bytes,
+                    cudaStream_t stream) {
+  const int T = a.T, r = a.lora.r;
+  if (!shape_ok(T, a.k, a.H, a.I, wtype)) return -1;
+  if (a.S <= 0 || a.S > EXPERT_CACHE_MAX_SLOTS || a.n_map < 0 || (a.map && a.n_map == 0))
+    return -1;
+  if (a.ldx < a.H || a.ldx % 8 || a.ldo < a.H) return -1;
+  if (T == 0) return 0;
+  if (!a.x || !a.ids || !a.weights || !a.w13 || !a.w2 || !a.out) return -1;
+  if ((wtype != kBf16) != (a.s13 != nullptr) || (wtype != kBf16) != (a.s2 != nullptr)) return -1;
+  if (misaligned(a.x, 16) || misaligned(a.w13, 16) || misaligned(a.w2, 16) ||
+      misaligned(a.out, 2) || misaligned(a.s13, 4) || misaligned(a.s2, 4) ||
+      misaligned(a.ids, 4) || misaligned(a.weights, 4) || misaligned(a.map, 4))
+    return -1;
+  const int per = tokens_per_launch(T, a.k, a.H, wtype);
+  const size_t need = carve(&a, nullptr, (size_t)per * a.k, a.I, wtype, r);
+  if (!workspace || misaligned(workspace, 256) || workspace_bytes < (long)need) return -1;
+  carve(&a, static_cast<unsigned char*>(workspace), (size_t)per * a.k, a.I, wtype, r);
+  const ExpertsArgs all = a;
+  for (int t = 0; t < T; t += per) {
+    a.T = T - t < per ? T - t : per;
+    a.x = all.x + t * all.ldx;
+    a.out = all.out + t * all.ldo;
+    a.ids = all.ids + (long long)t * all.k;
+    a.weights = all.weights + (long long)t * all.k;
+    if (r) a.lora.index = all.lora.index + t;
+    const int rc = wtype == kBf16   ? run_type<kBf16>(a, stream)
+                   : wtype == kInt8 ? run_type<kInt8>(a, stream)
+                                    : run_type<kFp8>(a, stream);
+    if (rc != 0) return rc;
+  }
+  return 0;
+}
+
+ExpertsArgs experts_args(const void* x, int T, int ldx, int H, const int* ids,
+                         const float* weights, int k, const int* expert_map, int n_map,
+                         const void* w13, const float* w13_scale, const void* w2,
+                         const float* w2_scale, int S, int I, void* out, int ldo) {
+  ExpertsArgs a{};
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.ids = ids;
+  a.weights = weights;
+  a.map = expert_map;
+  a.w13 = static_cast<const uint8_t*>(w13);
+  a.w2 = static_cast<const uint8_t*>(w2);
+  a.s13 = w13_scale;
+  a.s2 = w2_scale;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.ldx = ldx;
+  a.ldo = ldo;
+  a.T = T;
+  a.k = k;
+  a.H = H;
+  a.I = I;
+  a.S = S;
+  a.n_map = n_map;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int expert_cache_experts_workspace(int T, int k, int H, int I, int wtype, int r, long* bytes) {
+  if (!shape_ok(T, k, H, I, wtype) || bytes == nullptr) return -1;
+  if (r < 0 || r > EXPERT_CACHE_LORA_MAX_RANK || r % 8) return -1;
+  ExpertsArgs a{};
+  *bytes = T == 0 ? 0
+                  : (long)carve(&a, nullptr, (size_t)tokens_per_launch(T, k, H, wtype) * k, I,
+                                wtype, r);
+  return 0;
+}
+
+int expert_cache_experts(const void* x, int T, int ldx, int H, const int* ids,
+                         const float* weights, int k, const int* expert_map, int n_map,
+                         const void* w13, const float* w13_scale, const void* w2,
+                         const float* w2_scale, int wtype, int S, int I, void* out, int ldo,
+                         void* workspace, long workspace_bytes, cudaStream_t stream) {
+  return experts_checked(experts_args(x, T, ldx, H, ids, weights, k, expert_map, n_map, w13,
+                                      w13_scale, w2, w2_scale, S, I, out, ldo),
+                         wtype, workspace, workspace_bytes, stream);
+}
+
+int expert_cache_experts_lora(const void* x, int T, int ldx, int H, const int* ids,
+                              const float* weights, int k, const int* expert_map, int n_map,
+                              const void* w13, const float* w13_scale, const void* w2,
+                              const float* w2_scale, int wtype, int S, int I,
+                              const int* adapter, const void* a13, const void* b13,
+                              const void* a2, const void* b2, const float* scaling, int L,
+                              int E, int r, void* out, int ldo, void* workspace,
+                              long workspace_bytes, cudaStream_t stream) {
+  ExpertsArgs a = experts_args(x, T, ldx, H, ids, weights, k, expert_map, n_map, w13, w13_scale,
+                               w2, w2_scale, S, I, out, ldo);
+  if (L <= 0 || E <= 0 || r <= 0 || r > EXPERT_CACHE_LORA_MAX_RANK || r % 8) return -1;
+  if (!adapter || !a13 || !b13 || !a2 || !b2 || !scaling) return -1;
+  if (misaligned(a13, 16) || misaligned(b13, 16) || misaligned(a2, 16) || misaligned(b2, 16) ||
+      misaligned(adapter, 4) || misaligned(scaling, 4))
+    return -1;
+  a.lora.index = adapter;
+  a.lora.a13 = static_cast<const __nv_bfloat16*>(a13);
+  a.lora.b13 = static_cast<const __nv_bfloat16*>(b13);
+  a.lora.a2 = static_cast<const __nv_bfloat16*>(a2);
+  a.lora.b2 = static_cast<const __nv_bfloat16*>(b2);
+  a.lora.scaling = scaling;
+  a.lora.L = L;
+  a.lora.E = E;
+  a.lora.r = r;
+  return experts_checked(a, wtype, workspace, workspace_bytes, stream);
+}
+
+int expert_cache_route(const void* x, int T, int ldx, int H, const void* gate_w, int E, int k,
+                       int scoring, int renormalize, const float* bias, float scale,
+                       float* out_weights, int* out_ids, cudaStream_t stream) {
+  if (T < 0 || H <= 0 || H % 8 || H > EXPERT_CACHE_PREGATE_MAX_HIDDEN || ldx < H || ldx % 8)
+    return -1;
+  if (E <= 0 || E > EXPERT_CACHE_PREGATE_MAX_EXPERTS || k <= 0 || k > E ||
+      k > EXPERT_CACHE_EXPERTS_MAX_TOPK)
+    return -1;
+  if (scoring < 0 || scoring > 1 || (scoring == 0 && bias != nullptr)) return -1;
+  if (misaligned(x, 16) || misaligned(gate_w, 16) || misaligned(bias, 4) ||
+      misaligned(out_weights, 4) || misaligned(out_ids, 4))
+    return -1;
+  if (T == 0) return 0;
+  if (!x || !gate_w || !out_weights || !out_ids) return -1;
+  RouteArgs a{};
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.gate = static_cast<const __nv_bfloat16*>(gate_w);
+  a.bias = bias;
+  a.weights = out_weights;
+  a.ids = out_ids;
+  a.ldx = ldx;
+  a.T = T;
+  a.H = H;
+  a.E = E;
+  a.k = k;
+  a.sigmoid = scoring;
+  a.renorm = renormalize != 0;
+  a.scale = scale;
+  return launch(route_kernel, dim3(T), kRouteThreads, (size_t)E * 8, stream, a);
+}
+
+}  // extern "C"

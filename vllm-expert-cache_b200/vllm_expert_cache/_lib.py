@@ -4,7 +4,7 @@ Search order, as in the reference (vllm_expert_cache/_lib.py:17-33): $EXPERT_CAC
 then ``libexpertcache.so`` beside this package, then /usr/local/lib.  A missing library
 raises FileNotFoundError; there is no fallback path.  The handle is loaded once per
 process.  Argument types are the reference's (_lib.py:41-53) plus the fused-remap,
-expert-parallel, prefetch and single-launch step entry points this build adds.
+expert-parallel, prefetch, single-launch step and MoE-layer entry points this build adds.
 """
 
 from __future__ import annotations
@@ -18,7 +18,7 @@ GATHER_SLOTS = 6
 # Largest slot count of the single-launch step (EXPERT_CACHE_STEP_MAX_SLOTS).
 STEP_MAX_SLOTS = 256
 
-_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 MANAGE_ARGTYPES = [_P] + [_I] * 5 + [_P] * 8 + [_I] * 2 + [_P]
 MANAGE_REMAP_ARGTYPES = [_P] + [_I] * 5 + [_P] * 8 + [_I] * 2 + [_P, _I, _P]
 MANAGE_EP_ARGTYPES = [_P, _I, _P] + [_I] * 5 + [_P] * 8 + [_I] * 2 + [_P, _P]
@@ -27,6 +27,12 @@ PREGATE_ARGTYPES = [_P, _I, _I, _I, _P, _I, _I, _P, _P]
 GATHER_ARGTYPES = [_P, _P, _L] * GATHER_SLOTS + [_P, _P, _I, _I, _P]
 STEP_ARGTYPES = ([_P] + [_I] * 5 + [_P] * 8 + [_I] * 2 + [_P, _I] + [_P, _P, _L] * GATHER_SLOTS
                  + [_I, _I, _P, _I, _P])
+ROUTE_ARGTYPES = [_P, _I, _I, _I, _P] + [_I] * 4 + [_P, _F, _P, _P, _P]
+EXPERTS_ARGTYPES = ([_P, _I, _I, _I, _P, _P, _I, _P, _I] + [_P] * 4 + [_I] * 3
+                    + [_P, _I, _P, _L, _P])
+LORA_ARGTYPES = ([_P, _I, _I, _I, _P, _P, _I, _P, _I] + [_P] * 4 + [_I] * 3 + [_P] * 6
+                 + [_I] * 3 + [_P, _I, _P, _L, _P])
+EXPERTS_WORKSPACE_ARGTYPES = [_I] * 6 + [_P]
 
 _handle = None
 
@@ -62,6 +68,14 @@ def bind(h: ctypes.CDLL) -> ctypes.CDLL:
     h.expert_cache_gather.argtypes = GATHER_ARGTYPES
     h.expert_cache_step.restype = _I
     h.expert_cache_step.argtypes = STEP_ARGTYPES
+    h.expert_cache_route.restype = _I
+    h.expert_cache_route.argtypes = ROUTE_ARGTYPES
+    h.expert_cache_experts.restype = _I
+    h.expert_cache_experts.argtypes = EXPERTS_ARGTYPES
+    h.expert_cache_experts_lora.restype = _I
+    h.expert_cache_experts_lora.argtypes = LORA_ARGTYPES
+    h.expert_cache_experts_workspace.restype = _I
+    h.expert_cache_experts_workspace.argtypes = EXPERTS_WORKSPACE_ARGTYPES
     return h
 
 
