@@ -45,7 +45,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kMaxPairs = EXPERT_CACHE_MAX_SLOTS;   // (token, expert) pairs of one launch
 constexpr int kMaxTokens = 32;                      // tokens of one launch (4 column tiles)
 constexpr int kMaxCols = 16384;                     // pairs x padded tokens of one launch
-constexpr int kStageBytes = 112 * 1024;             // largest staged x
+constexpr size_t kSmem = 227 * 1024;                // shared memory of a CTA
 
 enum WType { kBf16 = 0, kInt8 = 1, kFp8 = 2 };
 
@@ -280,13 +280,45 @@ __device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, cons
   for (int i = 0; i < 4; ++i) mma_f16(c, a.lo[i], b.lo[i], a.hi[i], b.hi[i], w.lo[i], w.hi[i]);
 }
 
-__device__ __forceinline__ uint4 load_weights(const uint8_t* p) {
-  uint4 r;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-      : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-      : "l"(p));
-  return r;
+// ---------------------------------------------------------------------------------------
+// The stream of weights.  Every thread copies the very bytes that it will multiply into a
+// FIFO of its own in shared memory (cp.async, two 16-byte vectors a stage), so the stream
+// needs no barrier and no thread waits for another's data; kStages * 8 KB per SM are on
+// their way at any time, several times what the memory's latency asks for, which covers
+// the barriers and the tile ends too.
+
+constexpr int kStages = 16;
+constexpr int kFifoBytes = kStages * kThreads * 32;
+
+__device__ __forceinline__ void copy16(unsigned char* dst, const uint8_t* src, bool in) {
+  const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+  const int n = in ? 16 : 0;                   // 0: the vector is zero-filled, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n)
+               : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// The oldest of kStages committed stages has landed.
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+}
+struct Fifo {
+  unsigned char* base;       // this thread's vectors of stage 0
+  int put, get;
+  __device__ __forceinline__ explicit Fifo(unsigned char* smem)
+      : base(smem + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 16), put(0), get(0) {}
+  __device__ __forceinline__ unsigned char* slot(int i) const { return base + i * (kThreads * 32); }
+  __device__ __forceinline__ void push(const uint8_t* a, bool in_a, const uint8_t* b, bool in_b) {
+    copy16(slot(put), a, in_a);
+    copy16(slot(put) + 512, b, in_b);
+    put = put + 1 == kStages ? 0 : put + 1;
+  }
+  __device__ __forceinline__ void front(uint4* a, uint4* b) {
+    copy_wait();
+    *a = *reinterpret_cast<const uint4*>(slot(get));
+    *b = *reinterpret_cast<const uint4*>(slot(get) + 512);
+    get = get + 1 == kStages ? 0 : get + 1;
+  }
+};
 
 // ---------------------------------------------------------------------------------------
 // Quantised rows: q = round(v * Q / max|v|), scale = max|v| / Q.  The product v * Q of a
@@ -426,6 +458,18 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(const __grid_constant_
 template <int NT>
 constexpr int kRed = kWarps * 16 * 8 * NT;   // values in one buffer of the warps' partial sums
 
+// One tile: 8 consecutive row pairs of one entry (fewer at the end of the CTA's range or of
+// the entry).
+struct UpTile {
+  int row, e, i0, n;
+  __device__ __forceinline__ void at(int r, int r1, int I) {
+    row = r;
+    e = r / I;
+    i0 = r - e * I;
+    n = min(8, min(r1 - r, I - i0));
+  }
+};
+
 template <int WT, int NT>
 __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__ ExpertsArgs a,
                                                          int staged) {
@@ -433,8 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   using Acc = typename K::Acc;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  const Routing rt = routing_at(smem, P, NT);
-  Acc* red = reinterpret_cast<Acc*>(smem + routing_bytes(P, NT));
+  Fifo fifo(smem);
+  const Routing rt = routing_at(smem + kFifoBytes, P, NT);
+  Acc* red = reinterpret_cast<Acc*>(smem + kFifoBytes + routing_bytes(P, NT));
   float* xs = reinterpret_cast<float*>(red + 2 * kRed<NT>);
   unsigned char* st = reinterpret_cast<unsigned char*>(xs + kMaxTokens);
 
@@ -445,31 +490,55 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   const long long R = (long long)D * a.I;
   const int r0 = (int)(R * blockIdx.x / gridDim.x), r1 = (int)(R * (blockIdx.x + 1) / gridDim.x);
   if (r0 >= r1) return;
-  if (staged) {
-    stage_x<WT>(a, st, xs);
-    __syncthreads();
-  }
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int C = (a.H + K::kChunk - 1) / K::kChunk;
   const long long row_bytes = (long long)a.H * K::kItem;
+
+  // The warp's chunks of all tiles in order; `src` follows the stream's head.
+  UpTile head;
+  const uint8_t* src = nullptr;
+  int hc = warp;
+  const auto head_at = [&](int row) {
+    head.at(row, r1, a.I);
+    src = a.w13 + ((long long)rt.slot[head.e] * 2 * a.I + head.i0 + g) * row_bytes + q * 16;
+  };
+  const auto push = [&]() {
+    if (head.row < r1) {
+      const bool in = g < head.n && hc * K::kChunk + q * K::kVec < a.H;
+      fifo.push(src + hc * 64, in, src + a.I * row_bytes + hc * 64, in);
+      hc += kWarps;
+      if (hc >= C) {
+        hc = warp;
+        const int next = head.row + head.n;
+        if (next < r1) head_at(next);
+        else head.row = r1;
+      }
+    }
+    copy_commit();
+  };
+  head.row = r1;
+  if (warp < C) head_at(r0);
+  for (int i = 0; i < kStages; ++i) push();
+
+  if (staged) {
+    stage_x<WT>(a, st, xs);
+    __syncthreads();
+  }
   int buf = 0;
-  for (int row = r0, n; row < r1; row += n, buf ^= 1) {
-    const int e = row / a.I, i0 = row - e * a.I;
-    n = min(8, min(r1 - row, a.I - i0));
+  UpTile tile;
+  for (int row = r0; row < r1; row += tile.n, buf ^= 1) {
+    tile.at(row, r1, a.I);
+    const int e = tile.e, i0 = tile.i0, n = tile.n;
     const int slot = rt.slot[e];
     const unsigned mask = rt.mask[e];
-    const uint8_t* w = a.w13 + ((long long)slot * 2 * a.I + i0 + g) * row_bytes + q * 16;
     Acc acc[NT][4] = {};
     for (int c = warp; c < C; c += kWarps) {
-      uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
-      const bool in = c * K::kChunk + q * K::kVec < a.H;
-      if (g < n && in) {
-        wa = load_weights(w + c * 64);
-        wb = load_weights(w + a.I * row_bytes + c * 64);
-      }
+      uint4 wa, wb;
+      fifo.front(&wa, &wb);
       Wide fa, fb;
       if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
+      const bool in = c * K::kChunk + q * K::kVec < a.H;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (NT > 1 && !(mask >> nt & 1)) continue;
@@ -485,6 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
         if constexpr (WT == kInt8) chunk_mma_s8(acc[nt], wa, wb, v);
         if constexpr (WT == kFp8) chunk_mma_fp8(acc[nt], fa, fb, v);
       }
+      push();      // into the stage just read, whose vectors the products have taken
     }
     // partial sums of the warps: [warp][row][column]
     Acc* mine = red + buf * kRed<NT> + warp * 16 * 8 * NT;
@@ -542,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
 
 template <int WT>
 __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ ExpertsArgs a) {
+  release_dependents();       // down may start streaming: it waits for this kernel's end
   grid_dependency_wait();
-  release_dependents();
   const int p = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (slot_of(a, p) < 0) return;
   const size_t at = (size_t)p * a.I;
@@ -598,74 +668,149 @@ __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ E
 // ---------------------------------------------------------------------------------------
 // down
 
+// A chunk of one entry's rows [row, row + n) of the CTA; a warp takes every kWarps-th of a
+// row tile's D * C chunks.
+struct DownCursor {
+  int row, n, e, c;
+  __device__ __forceinline__ void start(int r, int r1, int C, int D) {
+    row = r;
+    n = min(16, r1 - r);
+    e = 0;
+    c = threadIdx.x >> 5;
+    wrap(C, D);
+  }
+  __device__ __forceinline__ void wrap(int C, int D) {
+    while (c >= C && e < D) { c -= C; ++e; }
+  }
+  // False at the end of the CTA's rows.
+  __device__ __forceinline__ bool settle(int r1, int C, int D) {
+    while (e >= D) {
+      if (row + n >= r1) return false;
+      start(row + n, r1, C, D);
+    }
+    return true;
+  }
+  __device__ __forceinline__ void next(int C, int D) {
+    c += kWarps;
+    wrap(C, D);
+  }
+};
+
+// The other operand of a chunk, in registers: read from L2 kAhead chunks ahead.
+template <int WT, int NT>
+struct DownOperand {
+  uint4 v[NT][WT == kBf16 ? 2 : 1];
+  float rf[2], cf[NT][2];       // 8-bit: scales of rows g, g + 8 and of columns 2q, 2q + 1
+};
+
 template <int WT, int NT>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  const Routing rt = routing_at(smem, P, NT);
-  float* red = reinterpret_cast<float*>(smem + routing_bytes(P, NT));
+  Fifo fifo(smem);
+  const Routing rt = routing_at(smem + kFifoBytes, P, NT);
+  float* red = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT));
 
-  grid_dependency_wait();
+  // Everything up to the wait reads the call's inputs only.  They are complete: this grid
+  // starts once every CTA of the kernels before it has passed its own wait.
   release_dependents();
   const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
   const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x);
-  if (r0 >= r1) return;
   build_routing<NT>(a, rt);
   const int D = rt.entries[0];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int C = (a.I + K::kChunk - 1) / K::kChunk;
   const long long row_bytes = (long long)a.I * K::kItem;
+
+  DownCursor head;
+  bool more = r0 < r1 && D > 0;
+  head.start(r0, r1, C, D);
+  const auto push = [&]() {
+    if (more && (more = head.settle(r1, C, D))) {
+      const bool in = head.c * K::kChunk + q * K::kVec < a.I;
+      const uint8_t* src = a.w2 + ((long long)rt.slot[head.e] * a.H + head.row + g) * row_bytes +
+                           head.c * 64 + q * 16;
+      fifo.push(src, in && g < head.n, src + 8 * row_bytes, in && g + 8 < head.n);
+      head.next(C, D);
+    }
+    copy_commit();
+  };
+  for (int i = 0; i < kStages; ++i) push();
+
+  grid_dependency_wait();
+  using Operand = DownOperand<WT, NT>;
+  constexpr int kAhead = NT == 4 ? 2 : 4;
+  const auto fetch = [&](const DownCursor& at, Operand& o) {
+    const bool in = at.c * K::kChunk + q * K::kVec < a.I;
+    if (WT != kBf16) {
+      const float* s2 = a.s2 + (long long)rt.slot[at.e] * a.H + at.row;
+      o.rf[0] = g < at.n ? s2[g] : 0.f;
+      o.rf[1] = g + 8 < at.n ? s2[g + 8] : 0.f;
+    }
+    const unsigned mask = rt.mask[at.e];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (NT > 1 && !(mask >> nt & 1)) continue;
+      const short* col = rt.col + (size_t)at.e * 8 * NT + nt * 8;
+      const int p = col[g];
+      const long long i = (long long)p * a.I + at.c * K::kChunk + q * K::kVec;
+      o.v[nt][0] = make_uint4(0, 0, 0, 0);
+      if constexpr (WT == kBf16) {
+        o.v[nt][1] = o.v[nt][0];
+        if (p >= 0 && in) {
+          o.v[nt][0] = __ldcg(reinterpret_cast<const uint4*>(a.h_hi + i));
+          o.v[nt][1] = __ldcg(reinterpret_cast<const uint4*>(a.h_lo + i));
+        }
+      } else {
+        if (p >= 0 && in) o.v[nt][0] = __ldcg(reinterpret_cast<const uint4*>(a.hq + i));
+        const int p0 = col[2 * q], p1 = col[2 * q + 1];
+        o.cf[nt][0] = p0 >= 0 ? __ldcg(a.h_scale + p0) : 0.f;
+        o.cf[nt][1] = p1 >= 0 ? __ldcg(a.h_scale + p1) : 0.f;
+      }
+    }
+  };
   for (int row = r0, n; row < r1; row += n) {
     n = min(16, r1 - row);
     float acc[NT][4] = {};
-    int e = 0, c = warp;
-    while (true) {
-      while (e < D && c >= C) { c -= C; ++e; }
-      if (e >= D) break;
-      const long long first = (long long)rt.slot[e] * a.H + row;
-      const unsigned mask = rt.mask[e];
-      const bool in = c * K::kChunk + q * K::kVec < a.I;
-      uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
-      if (in && g < n) wa = load_weights(a.w2 + (first + g) * row_bytes + c * 64 + q * 16);
-      if (in && g + 8 < n) wb = load_weights(a.w2 + (first + g + 8) * row_bytes + c * 64 + q * 16);
-      Wide fa, fb;
-      if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
-      float rf0 = 0.f, rf1 = 0.f;
-      if (WT != kBf16) {
-        if (g < n) rf0 = a.s2[first + g];
-        if (g + 8 < n) rf1 = a.s2[first + g + 8];
-      }
+    DownCursor at, ahead;
+    at.start(row, r1, C, D);
+    ahead = at;
+    Operand ops[kAhead];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (NT > 1 && !(mask >> nt & 1)) continue;
-        const short* col = rt.col + (size_t)e * 8 * NT + nt * 8;
-        const int p = col[g];
-        const long long at = (long long)p * a.I + c * K::kChunk + q * K::kVec;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if constexpr (WT == kBf16) {
-          uint4 v2 = v;
-          if (p >= 0 && in) {
-            v = *reinterpret_cast<const uint4*>(a.h_hi + at);
-            v2 = *reinterpret_cast<const uint4*>(a.h_lo + at);
+    for (int j = 0; j < kAhead; ++j)
+      if (ahead.e < D) { fetch(ahead, ops[j]); ahead.next(C, D); }
+    while (at.e < D) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (at.e >= D) break;
+        Operand& now = ops[j];
+        uint4 wa, wb;
+        fifo.front(&wa, &wb);
+        Wide fa, fb;
+        if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
+        const unsigned mask = rt.mask[at.e];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (NT > 1 && !(mask >> nt & 1)) continue;
+          if constexpr (WT == kBf16) {
+            chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][0]);
+            chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][1]);
+          } else {
+            typename K::Acc part[4] = {};
+            if constexpr (WT == kInt8) chunk_mma_s8(part, wa, wb, now.v[nt][0]);
+            if constexpr (WT == kFp8) chunk_mma_fp8(part, fa, fb, now.v[nt][0]);
+            acc[nt][0] += (float)part[0] * (now.rf[0] * now.cf[nt][0]);
+            acc[nt][1] += (float)part[1] * (now.rf[0] * now.cf[nt][1]);
+            acc[nt][2] += (float)part[2] * (now.rf[1] * now.cf[nt][0]);
+            acc[nt][3] += (float)part[3] * (now.rf[1] * now.cf[nt][1]);
           }
-          chunk_mma_bf16(acc[nt], wa, wb, v);
-          chunk_mma_bf16(acc[nt], wa, wb, v2);
-        } else {
-          if (p >= 0 && in) v = *reinterpret_cast<const uint4*>(a.hq + at);
-          const int p0 = col[2 * q], p1 = col[2 * q + 1];
-          const float c0 = p0 >= 0 ? a.h_scale[p0] : 0.f, c1 = p1 >= 0 ? a.h_scale[p1] : 0.f;
-          typename K::Acc part[4] = {};
-          if constexpr (WT == kInt8) chunk_mma_s8(part, wa, wb, v);
-          if constexpr (WT == kFp8) chunk_mma_fp8(part, fa, fb, v);
-          acc[nt][0] += (float)part[0] * (rf0 * c0);
-          acc[nt][1] += (float)part[1] * (rf0 * c1);
-          acc[nt][2] += (float)part[2] * (rf1 * c0);
-          acc[nt][3] += (float)part[3] * (rf1 * c1);
         }
+        push();
+        at.next(C, D);
+        if (ahead.e < D) { fetch(ahead, now); ahead.next(C, D); }
       }
-      c += kWarps;
     }
     float* mine = red + warp * 16 * 8 * NT;
 #pragma unroll
@@ -871,12 +1016,24 @@ size_t staged_bytes(int T, int H, int wtype) {
 
 int column_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
 
+// Shared memory of up_kernel without the copy of x; down_kernel needs less.
+size_t up_bytes(int P, int NT) {
+  return kFifoBytes + routing_bytes(P, NT) + 2 * (size_t)kWarps * 16 * 8 * NT * 4 +
+         kMaxTokens * 4;
+}
+
+// Does the copy of x fit beside it?  bf16 rows are read from L1 / L2 where it does not.
+bool fits_staged(int T, int k, int H, int wtype) {
+  const int NT = column_tiles(T);
+  return up_bytes(T * k, NT) + staged_bytes(T, H, wtype) <= kSmem;
+}
+
 // Tokens of one launch: as many as fit the column tiles, the pair tables and (8-bit
 // weights, which are multiplied by staged rows only) the shared memory.
 int tokens_per_launch(int T, int k, int H, int wtype) {
   int n = T < kMaxTokens ? T : kMaxTokens;
   while (n > 1 && (n * k > kMaxPairs || n * k * 8 * column_tiles(n) > kMaxCols ||
-                   (wtype != kBf16 && staged_bytes(n, H, wtype) > kStageBytes)))
+                   (wtype != kBf16 && !fits_staged(n, k, H, wtype))))
     --n;
   return n;
 }
@@ -921,18 +1078,15 @@ int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
                 stream, a);
     if (rc != 0) return rc;
   }
-  const size_t tables = routing_bytes(P, NT), red = (size_t)kRed<NT> * 4;
-  size_t stage = staged_bytes(a.T, a.H, WT);
-  const int staged = stage <= (size_t)kStageBytes;
-  if (!staged) stage = 0;
+  const int staged = fits_staged(a.T, a.k, a.H, WT);
   rc = launch(up_kernel<WT, NT>, dim3(sms), kThreads,
-              tables + 2 * red + kMaxTokens * 4 + stage, stream, a, staged);
+              up_bytes(P, NT) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a, staged);
   if (rc != 0) return rc;
   if (WT != kBf16 || a.lora.r) {
     rc = launch(mid_kernel<WT>, dim3(P), kThreads, 0, stream, a);
     if (rc != 0) return rc;
   }
-  return launch(down_kernel<WT, NT>, dim3(sms), kThreads, tables + red, stream, a);
+  return launch(down_kernel<WT, NT>, dim3(sms), kThreads, up_bytes(P, NT), stream, a);
 }
 
 template <int WT>
