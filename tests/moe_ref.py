@@ -66,7 +66,9 @@ def experts(x, weights, ids, w13, w2, s13=None, s2=None, expert_map=None, lora=N
                     b = b13[half * I:(half + 1) * I]
                     k = slice(half * r, (half + 1) * r)
                     gu[half * I:(half + 1) * I] += c * (b @ u[k])
-                    d[half * I:(half + 1) * I] += abs(c) * (H + r + 4) * EPS * (b.abs() @ um[k])
+                    # (A x and A2 h, like h, in 16 bits of mantissa)
+                    d[half * I:(half + 1) * I] += abs(c) * (
+                        (H + r + 4) * EPS + 2.0 ** -16) * (b.abs() @ um[k])
             g, up = gu[:I], gu[I:]
             act = g * torch.sigmoid(g)
             h = act * up
@@ -88,7 +90,7 @@ def experts(x, weights, ids, w13, w2, s13=None, s2=None, expert_map=None, lora=N
                 v = a2 @ h
                 y = y + c * (b2 @ v)
                 vm = a2.abs() @ h.abs()
-                dv = a2.abs() @ dh + (I + r + 4) * EPS * vm
+                dv = a2.abs() @ dh + ((I + r + 4) * EPS + 2.0 ** -16) * vm
                 dy = dy + abs(c) * (b2.abs() @ dv)
                 ym = ym + abs(c) * (b2.abs() @ vm)
             out[t] += wt * y

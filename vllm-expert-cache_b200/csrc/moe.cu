@@ -78,7 +78,8 @@ struct ExpertsArgs {
   float* h;                        // 8-bit weights: h [P][I]
   uint8_t* hq;                     // 8-bit weights: quantised h [P][I]
   float* h_scale;                  // 8-bit weights: its scale x weights[t,j] [P]
-  float *u, *v;                    // adapters: c A13 x [P][2r], c w A2 h [P][r]
+  __nv_bfloat16 *u_hi, *u_lo;      // adapters: c A13 x in two parts [P][2r]
+  __nv_bfloat16 *v_hi, *v_lo;      // adapters: c weights[t,j] A2 h in two parts [P][r]
   Adapters lora;
 };
 
@@ -88,19 +89,23 @@ struct ExpertsArgs {
 // an entry of its own for every repetition, so that a column never holds two pairs.
 
 struct Routing {
-  int* entries;          // [1]
+  int* entries;          // [0] entries, [1] does a token repeat a slot, [2] adapted pairs
   unsigned* bits;        // [kMaxPairs / 32] routed slots
   int* base;             // [kMaxPairs / 32] entries before a word of `bits`
   short* slot;           // [P] slot of an entry
   short* pair_slot;      // [P] slot of a pair, -1 = none
   unsigned char* mask;   // [P] column tiles of an entry with a pair in them
   short* col;            // [P][8 NT] pair of an entry's column, -1 = none
+  // with adapters
+  int* matrix;           // [P] a pair's index among the [L][E] adapter matrices, -1 = none
+  unsigned* adapted;     // [P] columns of an entry whose pair has an adapter
+  short* list;           // [P] the pairs with adapters
 };
 
 constexpr int kRoutingFixed = 16 + (kMaxPairs / 32) * 8;
 
-__host__ __device__ inline size_t routing_bytes(int P, int NT) {
-  return kRoutingFixed + ((size_t)P * (2 + 2 + 1 + 16 * NT) + 15) / 16 * 16;
+__host__ __device__ inline size_t routing_bytes(int P, int NT, bool lora) {
+  return kRoutingFixed + ((size_t)P * (2 + 2 + 1 + 16 * NT + (lora ? 10 : 0)) + 15) / 16 * 16 + 16;
 }
 
 __device__ __forceinline__ Routing routing_at(unsigned char* base, int P, int NT) {
@@ -112,6 +117,9 @@ __device__ __forceinline__ Routing routing_at(unsigned char* base, int P, int NT
   r.slot = r.col + (size_t)P * 8 * NT;
   r.pair_slot = r.slot + P;
   r.mask = reinterpret_cast<unsigned char*>(r.pair_slot + P);
+  r.matrix = reinterpret_cast<int*>(r.mask + (P + 15) / 16 * 16);
+  r.adapted = reinterpret_cast<unsigned*>(r.matrix + P);
+  r.list = reinterpret_cast<short*>(r.adapted + P);
   return r;
 }
 
@@ -121,19 +129,29 @@ __device__ __forceinline__ int slot_of(const ExpertsArgs& a, int p) {
   return (s >= 0 && s < a.S) ? s : -1;
 }
 
+// The index of a pair's adapter among the [L][E] matrices, or -1.
+__device__ __forceinline__ int matrix_of(const ExpertsArgs& a, int p) {
+  const int l = a.lora.index[p / a.k], e = a.ids[p];
+  return (l < 0 || l >= a.lora.L || e < 0 || e >= a.lora.E) ? -1 : l * a.lora.E + e;
+}
+
 // Whole CTA; ends with a barrier.  Entries are in ascending slot order (repetitions after
 // them in pair order), so sums over entries have one order.
-template <int NT>
+template <int NT, bool LORA>
 __device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
   const int P = a.T * a.k, tid = threadIdx.x;
   constexpr int kWords = kMaxPairs / 32;
   if (tid < kWords) r.bits[tid] = 0;
-  if (tid == 0) r.entries[1] = 0;       // set when some token repeats a slot
+  if (tid == 0) r.entries[1] = r.entries[2] = 0;
   for (int i = tid; i < P * 8 * NT / 2; i += kThreads)
     reinterpret_cast<int*>(r.col)[i] = -1;
   for (int p = tid; p < P; p += kThreads) {
     r.pair_slot[p] = (short)slot_of(a, p);
     r.mask[p] = 0;
+    if (LORA) {
+      r.matrix[p] = matrix_of(a, p);
+      r.adapted[p] = 0;
+    }
   }
   __syncthreads();
   bool again = false;
@@ -169,6 +187,7 @@ __device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
     const int t = p / a.k;
     r.slot[e] = (short)s;
     r.col[(size_t)e * 8 * NT + t] = (short)p;
+    if (LORA && r.matrix[p] >= 0) atomicOr(&r.adapted[e], 1u << t);
   }
   __syncthreads();
   if (repeats && tid == 0) {
@@ -180,9 +199,21 @@ __device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
       if (s < 0 || first) continue;
       r.slot[n] = (short)s;
       r.col[(size_t)n * 8 * NT + p / a.k] = (short)p;
+      if (LORA && r.matrix[p] >= 0) r.adapted[n] = 1u << p / a.k;
       ++n;
     }
     r.entries[0] = n;
+  }
+  if (LORA && tid < 32) {      // the adapted pairs in ascending order
+    int n = 0;
+    for (int at = 0; at < P; at += 32) {
+      const int p = at + tid;
+      const bool has = p < P && r.pair_slot[p] >= 0 && r.matrix[p] >= 0;
+      const unsigned b = __ballot_sync(0xffffffffu, has);
+      if (has) r.list[n + __popc(b & ((1u << tid) - 1u))] = (short)p;
+      n += __popc(b);
+    }
+    if (tid == 0) r.entries[2] = n;
   }
   if (repeats) __syncthreads();
   const int D = r.entries[0];
@@ -301,6 +332,18 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
 }
+// 16 bytes from L2, or zeros and no read.
+__device__ __forceinline__ uint4 load_or_zero(const void* p, bool in) {
+  uint4 r;
+  asm volatile(
+      "{.reg .pred p; setp.ne.b32 p, %5, 0; mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; "
+      "mov.b32 %3, 0; @p ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];}"
+      : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w)
+      : "l"(p), "r"((int)in)
+      : "memory");
+  return r;
+}
+
 struct Fifo {
   unsigned char* base;       // this thread's vectors of stage 0
   int put, get;
@@ -335,88 +378,94 @@ __device__ __forceinline__ float quant_scale(float top) {
   return top / (WT == kInt8 ? 127.f : 448.f);
 }
 
-// max |v| that keeps a NaN (fmaxf would drop it).
-__device__ __forceinline__ float max_abs(float m, float v) {
-  v = fabsf(v);
-  return (v > m || v != v) ? v : m;
+// The bits of |v| order as |v| does, a NaN above all, so that a maximum of them keeps it.
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float clamp_top(unsigned bits) {
+  const float m = __uint_as_float(bits);
+  return m < 1e-10f ? 1e-10f : m;
 }
-__device__ __forceinline__ float warp_max_abs(float m) {
-#pragma unroll
-  for (int off = 16; off; off >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, off));
-  return m;
-}
-__device__ __forceinline__ float clamp_top(float m) { return m < 1e-10f ? 1e-10f : m; }
 
 // x of the CTA's tokens in shared memory as [chunk][T][64 bytes] (zeros past H), quantised
-// for 8-bit weights with the scales in `xs`.  A warp takes a token.  No barrier.
+// for 8-bit weights with the scales in `xs`.  Whole CTA; ends with a barrier.
 template <int WT>
 __device__ void stage_x(const ExpertsArgs& a, unsigned char* st, float* xs) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kChunk = Kind<WT>::kChunk, kVec = Kind<WT>::kVec;
-  const int C = (a.H + kChunk - 1) / kChunk;
-  for (int t = warp; t < a.T; t += kWarps) {
-    const __nv_bfloat16* x = a.x + t * a.ldx;
-    float top = 0.f;
-    if (WT != kBf16) {
-      for (int i = lane * 8; i < a.H; i += 256) {
-        const uint4 v = *reinterpret_cast<const uint4*>(x + i);
-        const unsigned u[4] = {v.x, v.y, v.z, v.w};
+  if (WT != kBf16) {
+    __shared__ unsigned tops[kMaxTokens];
+    if (tid < kMaxTokens) tops[tid] = 0;
+    __syncthreads();
+    const int segs = (a.H + 511) / 512;           // a warp takes 512 columns of a token
+    for (int i = warp; i < segs * a.T; i += kWarps) {
+      const int t = i / segs, at = (i - t * segs) * 512 + lane * 8;
+      const __nv_bfloat16* x = a.x + t * a.ldx + at;
+      uint4 v[2] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          top = max_abs(top, __uint_as_float(u[j] << 16));
-          top = max_abs(top, __uint_as_float(u[j] & 0xffff0000u));
-        }
+      for (int j = 0; j < 2; ++j)
+        if (at + j * 256 < a.H) v[j] = *reinterpret_cast<const uint4*>(x + j * 256);
+      unsigned top = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          top = max(top, max(u[m] << 16 & 0x7fffffffu, u[m] & 0x7fff0000u));
       }
-      top = clamp_top(warp_max_abs(top));
-      if (lane == 0) xs[t] = quant_scale<WT>(top);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&tops[t], top);
     }
-    for (int i = lane; i < C * 4; i += 32) {       // 16-byte pieces
-      uint4 o = make_uint4(0, 0, 0, 0);
-      if (i * kVec < a.H) {
-        const uint4* src = reinterpret_cast<const uint4*>(x + i * kVec);
-        if (WT == kBf16) {
-          o = src[0];
-        } else {
-          unsigned w[4];
+    __syncthreads();
+    if (tid < a.T) xs[tid] = clamp_top(tops[tid]);
+    __syncthreads();
+  }
+  const int pieces = (a.H + kChunk - 1) / kChunk * 4;        // 16 bytes each, of a token
+  for (int i = tid; i < pieces * a.T; i += kThreads) {
+    const int t = i / pieces, m = i - t * pieces;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (m * kVec < a.H) {
+      const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.ldx + m * kVec);
+      if (WT == kBf16) {
+        o = src[0];
+      } else {
+        const float top = xs[t];
+        unsigned w[4];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4 v = src[half];
-            const unsigned u[4] = {v.x, v.y, v.z, v.w};
+        for (int half = 0; half < 2; ++half) {
+          const uint4 v = src[half];
+          const unsigned u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              w[2 * half + j] =
-                  quantise<WT>(__uint_as_float(u[2 * j] << 16), top) |
-                  quantise<WT>(__uint_as_float(u[2 * j] & 0xffff0000u), top) << 8 |
-                  quantise<WT>(__uint_as_float(u[2 * j + 1] << 16), top) << 16 |
-                  quantise<WT>(__uint_as_float(u[2 * j + 1] & 0xffff0000u), top) << 24;
-          }
-          o = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int j = 0; j < 2; ++j)
+            w[2 * half + j] =
+                quantise<WT>(__uint_as_float(u[2 * j] << 16), top) |
+                quantise<WT>(__uint_as_float(u[2 * j] & 0xffff0000u), top) << 8 |
+                quantise<WT>(__uint_as_float(u[2 * j + 1] << 16), top) << 16 |
+                quantise<WT>(__uint_as_float(u[2 * j + 1] & 0xffff0000u), top) << 24;
         }
+        o = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      *reinterpret_cast<uint4*>(st + ((size_t)(i >> 2) * a.T + t) * 64 + (i & 3) * 16) = o;
     }
+    *reinterpret_cast<uint4*>(st + ((size_t)(m >> 2) * a.T + t) * 64 + (m & 3) * 16) = o;
+  }
+  __syncthreads();
+  if (WT != kBf16) {
+    if (tid < a.T) xs[tid] = quant_scale<WT>(xs[tid]);
+    __syncthreads();
   }
 }
 
-// The adapter of a pair, or -1; *matrix = its index among the [L][E] adapter matrices.
-__device__ __forceinline__ int adapter_of(const ExpertsArgs& a, int p, long long* matrix) {
-  const int t = p / a.k, l = a.lora.index[t], e = a.ids[p];
-  if (l < 0 || l >= a.lora.L || e < 0 || e >= a.lora.E) return -1;
-  *matrix = (long long)l * a.lora.E + e;
-  return l;
+// A sum as two bf16 values (an infinite high part has no remainder).
+__device__ __forceinline__ void split(float v, __nv_bfloat16* hi, __nv_bfloat16* lo) {
+  *hi = __float2bfloat16(v);
+  const float back = __bfloat162float(*hi);
+  *lo = __float2bfloat16(isfinite(back) ? v - back : 0.f);
 }
 
-// sum_j b[j] * u[j], r a multiple of 8, b 16-byte aligned bf16, u fp32.
-__device__ __forceinline__ float dot_row(const __nv_bfloat16* b, const float* u, int r) {
-  float s = 0.f;
-  for (int j = 0; j < r; j += 8) {
-    const uint4 v = *reinterpret_cast<const uint4*>(b + j);
-    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
+  const unsigned x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s += __uint_as_float(w[i] << 16) * u[j + 2 * i];
-      s += __uint_as_float(w[i] & 0xffff0000u) * u[j + 2 * i + 1];
-    }
+  for (int j = 0; j < 4; ++j) {
+    s = fmaf(__uint_as_float(x[j] << 16), __uint_as_float(y[j] << 16), s);
+    s = fmaf(__uint_as_float(x[j] & 0xffff0000u), __uint_as_float(y[j] & 0xffff0000u), s);
   }
   return s;
 }
@@ -430,47 +479,43 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(const __grid_constant_
   const int p = blockIdx.x, lane = threadIdx.x & 31;
   const int row = blockIdx.y * kWarps + (threadIdx.x >> 5);
   const int rows = 2 * a.lora.r;
-  long long m;
   if (row >= rows || slot_of(a, p) < 0) return;
-  const int l = adapter_of(a, p, &m);
-  if (l < 0) return;
-  const __nv_bfloat16* w = a.lora.a13 + (m * rows + row) * a.H;
+  const int m = matrix_of(a, p);
+  if (m < 0) return;
+  const __nv_bfloat16* w = a.lora.a13 + ((long long)m * rows + row) * a.H;
   const __nv_bfloat16* x = a.x + (p / a.k) * a.ldx;
   float s = 0.f;
-  for (int i = lane * 8; i < a.H; i += 256) {
-    const uint4 wv = *reinterpret_cast<const uint4*>(w + i);
-    const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
-    const unsigned ww[4] = {wv.x, wv.y, wv.z, wv.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s += __uint_as_float(ww[j] << 16) * __uint_as_float(xw[j] << 16);
-      s += __uint_as_float(ww[j] & 0xffff0000u) * __uint_as_float(xw[j] & 0xffff0000u);
-    }
-  }
+#pragma unroll 8
+  for (int i = lane * 8; i < a.H; i += 256)
+    s = dot8(*reinterpret_cast<const uint4*>(w + i), *reinterpret_cast<const uint4*>(x + i), s);
 #pragma unroll
   for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  if (lane == 0) a.u[(size_t)p * rows + row] = s * a.lora.scaling[l];
+  if (lane == 0) {
+    const size_t at = (size_t)p * rows + row;
+    split(s * a.lora.scaling[m / a.lora.E], a.u_hi + at, a.u_lo + at);
+  }
 }
 
 // ---------------------------------------------------------------------------------------
 // up
 
-template <int NT>
-constexpr int kRed = kWarps * 16 * 8 * NT;   // values in one buffer of the warps' partial sums
-
-// One tile: 8 consecutive row pairs of one entry (fewer at the end of the CTA's range or of
-// the entry).
+// A warp's share of the flat range of all entries' row pairs, in tiles of up to 8 rows of one
+// entry.  No warp waits for another: the tile's rows stay in one warp over their whole
+// length, so that h comes straight from the accumulators.  (Splitting a tile's columns over
+// the CTA's warps, with a barrier and a sum at every tile's end, was 1.4 times slower for
+// one token in int8.)
 struct UpTile {
   int row, e, i0, n;
   __device__ __forceinline__ void at(int r, int r1, int I) {
     row = r;
     e = r / I;
     i0 = r - e * I;
-    n = min(8, min(r1 - r, I - i0));
+    const int left = min(r1 - r, I - i0), tiles = (left + 7) / 8;
+    n = (left + tiles - 1) / tiles;
   }
 };
 
-template <int WT, int NT>
+template <int WT, int NT, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__ ExpertsArgs a,
                                                          int staged) {
   using K = Kind<WT>;
@@ -479,37 +524,51 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   const int P = a.T * a.k;
   Fifo fifo(smem);
   const Routing rt = routing_at(smem + kFifoBytes, P, NT);
-  Acc* red = reinterpret_cast<Acc*>(smem + kFifoBytes + routing_bytes(P, NT));
-  float* xs = reinterpret_cast<float*>(red + 2 * kRed<NT>);
+  float* xs = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT, LORA));
   unsigned char* st = reinterpret_cast<unsigned char*>(xs + kMaxTokens);
 
-  grid_dependency_wait();
+  // With adapters shrink_kernel runs before this one; it starts this grid once its own wait
+  // is over, so the call's inputs are complete and only its result is waited for, below.
+  if (!LORA) grid_dependency_wait();
   release_dependents();
-  build_routing<NT>(a, rt);
+  build_routing<NT, LORA>(a, rt);
   const int D = rt.entries[0];
-  const long long R = (long long)D * a.I;
-  const int r0 = (int)(R * blockIdx.x / gridDim.x), r1 = (int)(R * (blockIdx.x + 1) / gridDim.x);
-  if (r0 >= r1) return;
-
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const long long R = (long long)D * a.I, W = (long long)gridDim.x * kWarps;
+  const int w = blockIdx.x * kWarps + warp;
+  const int r0 = (int)(R * w / W), r1 = (int)(R * (w + 1) / W);
   const int C = (a.H + K::kChunk - 1) / K::kChunk;
+  const int RC = LORA ? (a.lora.r + 31) / 32 : 0;
   const long long row_bytes = (long long)a.H * K::kItem;
 
-  // The warp's chunks of all tiles in order; `src` follows the stream's head.
+  // The chunks of the warp's tiles in order, each tile's adapted columns after them; `src`
+  // and the counters follow the head of the stream.
   UpTile head;
   const uint8_t* src = nullptr;
-  int hc = warp;
+  int hc = 0, hr = 0;
+  unsigned left = 0;
   const auto head_at = [&](int row) {
     head.at(row, r1, a.I);
     src = a.w13 + ((long long)rt.slot[head.e] * 2 * a.I + head.i0 + g) * row_bytes + q * 16;
+    hc = 0;
+    if (LORA) left = rt.adapted[head.e];
   };
   const auto push = [&]() {
     if (head.row < r1) {
-      const bool in = g < head.n && hc * K::kChunk + q * K::kVec < a.H;
-      fifo.push(src + hc * 64, in, src + a.I * row_bytes + hc * 64, in);
-      hc += kWarps;
-      if (hc >= C) {
-        hc = warp;
+      if (hc < C) {
+        const bool in = g < head.n && hc * K::kChunk + q * K::kVec < a.H;
+        fifo.push(src + hc * 64, in, src + a.I * row_bytes + hc * 64, in);
+        ++hc;
+      } else if (LORA) {
+        const int p = rt.col[(size_t)head.e * 8 * NT + __ffs(left) - 1];
+        const bool in = g < head.n && hr * 32 + q * 8 < a.lora.r;
+        const __nv_bfloat16* b = a.lora.b13 + ((long long)rt.matrix[p] * 2 * a.I + head.i0 + g) *
+                                                  a.lora.r + hr * 32 + q * 8;
+        fifo.push(reinterpret_cast<const uint8_t*>(b), in,
+                  reinterpret_cast<const uint8_t*>(b + (long long)a.I * a.lora.r), in);
+        if (++hr == RC) { hr = 0; left &= left - 1; }
+      }
+      if (hc >= C && (!LORA || left == 0)) {
         const int next = head.row + head.n;
         if (next < r1) head_at(next);
         else head.row = r1;
@@ -518,22 +577,27 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
     copy_commit();
   };
   head.row = r1;
-  if (warp < C) head_at(r0);
+  if (r0 < r1) head_at(r0);
   for (int i = 0; i < kStages; ++i) push();
 
-  if (staged) {
-    stage_x<WT>(a, st, xs);
-    __syncthreads();
-  }
-  int buf = 0;
+  if (staged) stage_x<WT>(a, st, xs);
+  if (LORA) grid_dependency_wait();
+
   UpTile tile;
-  for (int row = r0; row < r1; row += tile.n, buf ^= 1) {
+  for (int row = r0; row < r1; row += tile.n) {
     tile.at(row, r1, a.I);
-    const int e = tile.e, i0 = tile.i0, n = tile.n;
-    const int slot = rt.slot[e];
-    const unsigned mask = rt.mask[e];
+    const int slot = rt.slot[tile.e], r = tile.i0 + g;
+    const unsigned mask = rt.mask[tile.e];
+    const bool mine = g < tile.n;
+    const short* col = rt.col + (size_t)tile.e * 8 * NT;
+    float sg = 1.f, su = 1.f;
+    if (WT != kBf16 && mine) {
+      sg = a.s13[(long long)slot * 2 * a.I + r];
+      su = a.s13[(long long)slot * 2 * a.I + a.I + r];
+    }
     Acc acc[NT][4] = {};
-    for (int c = warp; c < C; c += kWarps) {
+#pragma unroll 2
+    for (int c = 0; c < C; ++c) {
       uint4 wa, wb;
       fifo.front(&wa, &wb);
       Wide fa, fb;
@@ -556,52 +620,57 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       }
       push();      // into the stage just read, whose vectors the products have taken
     }
-    // partial sums of the warps: [warp][row][column]
-    Acc* mine = red + buf * kRed<NT> + warp * 16 * 8 * NT;
+    // Adapters: one more product for each adapted column, B13's rows with u in that column
+    // alone.  Gate and up have different u, so each takes its half of the 16 rows.
+    float add[LORA ? NT : 1][4] = {};
+    if (LORA) {
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      for (unsigned cols = rt.adapted[tile.e]; cols; cols &= cols - 1) {
+        const int t = __ffs(cols) - 1;
+        const size_t at = (size_t)col[t] * 2 * a.lora.r + q * 8;
+        for (int rc = 0; rc < RC; ++rc) {
+          const bool has = g == (t & 7) && rc * 32 + q * 8 < a.lora.r;
+          const uint4 v[4] = {load_or_zero(a.u_hi + at + rc * 32, has),
+                              load_or_zero(a.u_lo + at + rc * 32, has),
+                              load_or_zero(a.u_hi + at + a.lora.r + rc * 32, has),
+                              load_or_zero(a.u_lo + at + a.lora.r + rc * 32, has)};
+          uint4 wa, wb;
+          fifo.front(&wa, &wb);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            // (a product with zeros in the other column tiles: a branch around it would
+            // index the accumulators at run time and put them into local memory)
+            const bool here = NT == 1 || t >> 3 == nt;
+            chunk_mma_bf16(add[nt], wa, zero, here ? v[0] : zero);
+            chunk_mma_bf16(add[nt], wa, zero, here ? v[1] : zero);
+            chunk_mma_bf16(add[nt], zero, wb, here ? v[2] : zero);
+            chunk_mma_bf16(add[nt], zero, wb, here ? v[3] : zero);
+          }
+          push();
+        }
+      }
+    }
+    if (!mine) continue;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int c = nt * 8 + 2 * q;
-      mine[g * 8 * NT + c] = acc[nt][0];
-      mine[g * 8 * NT + c + 1] = acc[nt][1];
-      mine[(g + 8) * 8 * NT + c] = acc[nt][2];
-      mine[(g + 8) * 8 * NT + c + 1] = acc[nt][3];
-    }
-    __syncthreads();
-    for (int o = tid; o < 8 * a.T; o += kThreads) {
-      const int i = o & 7, t = o >> 3;
-      const int p = rt.col[(size_t)e * 8 * NT + t];
-      if (i >= n || p < 0) continue;
-      const Acc* src = red + buf * kRed<NT> + i * 8 * NT + t;
-      Acc sg = 0, su = 0;
+      if (NT > 1 && !(mask >> nt & 1)) continue;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        sg += src[k * 16 * 8 * NT];
-        su += src[(k * 16 + 8) * 8 * NT];
-      }
-      float gate = (float)sg, up = (float)su;
-      const int r = i0 + i;
-      if (WT != kBf16) {
-        gate *= xs[t] * a.s13[(long long)slot * 2 * a.I + r];
-        up *= xs[t] * a.s13[(long long)slot * 2 * a.I + a.I + r];
-      }
-      long long m;
-      if (a.lora.r && adapter_of(a, p, &m) >= 0) {
-        const __nv_bfloat16* b = a.lora.b13 + (m * 2 * a.I + r) * a.lora.r;
-        const float* u = a.u + (size_t)p * 2 * a.lora.r;
-        gate += dot_row(b, u, a.lora.r);
-        up += dot_row(b + (long long)a.I * a.lora.r, u + a.lora.r, a.lora.r);
-      }
-      float h = gate / (1.f + expf(-gate)) * up;
-      if (WT == kBf16) {
-        h *= a.weights[p];
-        const __nv_bfloat16 hi = __float2bfloat16(h);
-        const float back = __bfloat162float(hi);
-        // (an infinite hi has no remainder)
-        const __nv_bfloat16 lo = __float2bfloat16(isfinite(back) ? h - back : 0.f);
-        a.h_hi[(size_t)p * a.I + r] = hi;
-        a.h_lo[(size_t)p * a.I + r] = lo;
-      } else {
-        a.h[(size_t)p * a.I + r] = h;
+      for (int j = 0; j < 2; ++j) {
+        const int t = nt * 8 + 2 * q + j, p = col[t];
+        if (p < 0) continue;
+        float gate = (float)acc[nt][j], up = (float)acc[nt][2 + j];
+        if (WT != kBf16) {
+          gate *= xs[t] * sg;
+          up *= xs[t] * su;
+        }
+        if (LORA) {
+          gate += add[nt][j];
+          up += add[nt][2 + j];
+        }
+        const float h = gate / (1.f + expf(-gate)) * up;
+        const size_t at = (size_t)p * a.I + r;
+        if (WT == kBf16) split(h * a.weights[p], a.h_hi + at, a.h_lo + at);
+        else a.h[at] = h;
       }
     }
   }
@@ -610,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------------------
 // mid: one CTA per pair
 
-template <int WT>
+template <int WT, bool LORA>
 __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ ExpertsArgs a) {
   release_dependents();       // down may start streaming: it waits for this kernel's end
   grid_dependency_wait();
@@ -618,131 +687,174 @@ __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ E
   if (slot_of(a, p) < 0) return;
   const size_t at = (size_t)p * a.I;
   if (WT != kBf16) {
-    __shared__ float tops[kWarps];
-    float top = 0.f;
+    __shared__ unsigned tops[kWarps];
+    unsigned top = 0;
     for (int i = tid * 4; i < a.I; i += kThreads * 4) {
-      const float4 v = *reinterpret_cast<const float4*>(a.h + at + i);
-      top = max_abs(max_abs(max_abs(max_abs(top, v.x), v.y), v.z), v.w);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
+      top = max(max(top, max(abs_bits(v.x), abs_bits(v.y))), max(abs_bits(v.z), abs_bits(v.w)));
     }
-    top = warp_max_abs(top);
+    top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = max_abs(top, tops[w]);
-    top = clamp_top(top);
-    if (tid == 0) a.h_scale[p] = quant_scale<WT>(top) * a.weights[p];
+    for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
+    const float m = clamp_top(top);
+    if (tid == 0) a.h_scale[p] = quant_scale<WT>(m) * a.weights[p];
     for (int i = tid * 4; i < a.I; i += kThreads * 4) {
-      const float4 v = *reinterpret_cast<const float4*>(a.h + at + i);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
       *reinterpret_cast<unsigned*>(a.hq + at + i) =
-          quantise<WT>(v.x, top) | quantise<WT>(v.y, top) << 8 | quantise<WT>(v.z, top) << 16 |
-          quantise<WT>(v.w, top) << 24;
+          quantise<WT>(v.x, m) | quantise<WT>(v.y, m) << 8 | quantise<WT>(v.z, m) << 16 |
+          quantise<WT>(v.w, m) << 24;
     }
   }
-  long long m;
-  if (a.lora.r == 0) return;
-  const int l = adapter_of(a, p, &m);
-  if (l < 0) return;
+  if (!LORA) return;
+  const int m = matrix_of(a, p);
+  if (m < 0) return;
   for (int row = warp; row < a.lora.r; row += kWarps) {
-    const __nv_bfloat16* w = a.lora.a2 + (m * a.lora.r + row) * a.I;
+    const __nv_bfloat16* w = a.lora.a2 + ((long long)m * a.lora.r + row) * a.I;
     float s = 0.f;
+#pragma unroll 4
     for (int i = lane * 8; i < a.I; i += 256) {
       const uint4 wv = *reinterpret_cast<const uint4*>(w + i);
-      const unsigned ww[4] = {wv.x, wv.y, wv.z, wv.w};
+      if (WT == kBf16) {
+        s = dot8(wv, __ldcg(reinterpret_cast<const uint4*>(a.h_hi + at + i)), s);
+        s = dot8(wv, __ldcg(reinterpret_cast<const uint4*>(a.h_lo + at + i)), s);
+      } else {
+        const float4 h0 = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
+        const float4 h1 = __ldcg(reinterpret_cast<const float4*>(a.h + at + i + 4));
+        const unsigned x[4] = {wv.x, wv.y, wv.z, wv.w};
+        const float h[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float h = WT == kBf16 ? __bfloat162float(a.h_hi[at + i + j]) +
-                                          __bfloat162float(a.h_lo[at + i + j])
-                                    : a.h[at + i + j];
-        s += __uint_as_float(j & 1 ? ww[j / 2] & 0xffff0000u : ww[j / 2] << 16) * h;
+        for (int j = 0; j < 4; ++j) {
+          s = fmaf(__uint_as_float(x[j] << 16), h[2 * j], s);
+          s = fmaf(__uint_as_float(x[j] & 0xffff0000u), h[2 * j + 1], s);
+        }
       }
     }
 #pragma unroll
     for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    // bf16 weights: h already carries the routing weight
-    if (lane == 0)
-      a.v[(size_t)p * a.lora.r + row] =
-          s * a.lora.scaling[l] * (WT == kBf16 ? 1.f : a.weights[p]);
+    if (lane == 0) {
+      const size_t to = (size_t)p * a.lora.r + row;
+      // bf16 weights: h already carries the routing weight
+      s *= a.lora.scaling[m / a.lora.E] * (WT == kBf16 ? 1.f : a.weights[p]);
+      split(s, a.v_hi + to, a.v_lo + to);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // down
 
-// A chunk of one entry's rows [row, row + n) of the CTA; a warp takes every kWarps-th of a
-// row tile's D * C chunks.
+// Where a warp is in the stream of a CTA's rows: a tile of up to 16 rows after the other, in
+// each the C chunks of every entry and then, as entries from D on, the RC chunks of every
+// adapted pair; the warps take these chunks in turn.
 struct DownCursor {
   int row, n, e, c;
-  __device__ __forceinline__ void start(int r, int r1, int C, int D) {
+  int r1, C, D, RC, N;       // N = entries + adapted pairs
+  __device__ __forceinline__ void start(int r) {
     row = r;
-    n = min(16, r1 - r);
+    const int left = r1 - r, tiles = (left + 15) / 16;
+    n = tiles ? (left + tiles - 1) / tiles : 0;
     e = 0;
     c = threadIdx.x >> 5;
-    wrap(C, D);
+    wrap();
   }
-  __device__ __forceinline__ void wrap(int C, int D) {
-    while (c >= C && e < D) { c -= C; ++e; }
+  __device__ __forceinline__ void wrap() {
+    while (e < N && c >= (e < D ? C : RC)) { c -= e < D ? C : RC; ++e; }
   }
-  // False at the end of the CTA's rows.
-  __device__ __forceinline__ bool settle(int r1, int C, int D) {
-    while (e >= D) {
+  __device__ __forceinline__ bool in_tile() const { return e < N; }
+  // On to the next tile where this one is done; false after the last.
+  __device__ __forceinline__ bool settle() {
+    while (e >= N) {
       if (row + n >= r1) return false;
-      start(row + n, r1, C, D);
+      start(row + n);
     }
     return true;
   }
-  __device__ __forceinline__ void next(int C, int D) {
+  __device__ __forceinline__ void next() {
     c += kWarps;
-    wrap(C, D);
+    wrap();
   }
 };
 
 // The other operand of a chunk, in registers: read from L2 kAhead chunks ahead.
-template <int WT, int NT>
+template <int WT, int NT, bool LORA>
 struct DownOperand {
-  uint4 v[NT][WT == kBf16 ? 2 : 1];
+  uint4 v[NT][WT == kBf16 || LORA ? 2 : 1];
   float rf[2], cf[NT][2];       // 8-bit: scales of rows g, g + 8 and of columns 2q, 2q + 1
 };
 
-template <int WT, int NT>
+template <int NT>
+constexpr int kRed = kWarps * 16 * 8 * NT;   // the warps' partial sums
+
+template <int WT, int NT, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
   Fifo fifo(smem);
   const Routing rt = routing_at(smem + kFifoBytes, P, NT);
-  float* red = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT));
+  float* red = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT, LORA));
 
   // Everything up to the wait reads the call's inputs only.  They are complete: this grid
-  // starts once every CTA of the kernels before it has passed its own wait.
+  // starts once every CTA of the kernels before it has started, the first of them after its
+  // own wait.
   release_dependents();
   const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
   const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x);
-  build_routing<NT>(a, rt);
+  build_routing<NT, LORA>(a, rt);
   const int D = rt.entries[0];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int C = (a.I + K::kChunk - 1) / K::kChunk;
   const long long row_bytes = (long long)a.I * K::kItem;
 
   DownCursor head;
-  bool more = r0 < r1 && D > 0;
-  head.start(r0, r1, C, D);
+  head.r1 = r1;
+  head.C = (a.I + K::kChunk - 1) / K::kChunk;
+  head.D = D;
+  head.RC = LORA ? (a.lora.r + 31) / 32 : 1;
+  head.N = D + (LORA ? rt.entries[2] : 0);
+  bool more = r0 < r1 && head.N > 0;
+  head.start(r0);
   const auto push = [&]() {
-    if (more && (more = head.settle(r1, C, D))) {
-      const bool in = head.c * K::kChunk + q * K::kVec < a.I;
-      const uint8_t* src = a.w2 + ((long long)rt.slot[head.e] * a.H + head.row + g) * row_bytes +
-                           head.c * 64 + q * 16;
-      fifo.push(src, in && g < head.n, src + 8 * row_bytes, in && g + 8 < head.n);
-      head.next(C, D);
+    if (more && (more = head.settle())) {
+      if (!LORA || head.e < D) {
+        const bool in = head.c * K::kChunk + q * K::kVec < a.I;
+        const uint8_t* src =
+            a.w2 + ((long long)rt.slot[head.e] * a.H + head.row + g) * row_bytes + head.c * 64 +
+            q * 16;
+        fifo.push(src, in && g < head.n, src + 8 * row_bytes, in && g + 8 < head.n);
+      } else {
+        const int p = rt.list[head.e - D];
+        const bool in = head.c * 32 + q * 8 < a.lora.r;
+        const __nv_bfloat16* b = a.lora.b2 + ((long long)rt.matrix[p] * a.H + head.row + g) *
+                                                 a.lora.r + head.c * 32 + q * 8;
+        fifo.push(reinterpret_cast<const uint8_t*>(b), in && g < head.n,
+                  reinterpret_cast<const uint8_t*>(b + 8 * a.lora.r), in && g + 8 < head.n);
+      }
+      head.next();
     }
     copy_commit();
   };
+  DownCursor at = head;
   for (int i = 0; i < kStages; ++i) push();
 
   grid_dependency_wait();
-  using Operand = DownOperand<WT, NT>;
+  using Operand = DownOperand<WT, NT, LORA>;
   constexpr int kAhead = NT == 4 ? 2 : 4;
   const auto fetch = [&](const DownCursor& at, Operand& o) {
+    if (LORA && at.e >= D) {
+      const int p = rt.list[at.e - D], t = p / a.k;
+      const size_t i = (size_t)p * a.lora.r + at.c * 32 + q * 8;
+      const bool in = g == (t & 7) && at.c * 32 + q * 8 < a.lora.r;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const bool here = in && (NT == 1 || t >> 3 == nt);
+        o.v[nt][0] = load_or_zero(a.v_hi + i, here);
+        o.v[nt][LORA] = load_or_zero(a.v_lo + i, here);
+      }
+      return;
+    }
     const bool in = at.c * K::kChunk + q * K::kVec < a.I;
     if (WT != kBf16) {
       const float* s2 = a.s2 + (long long)rt.slot[at.e] * a.H + at.row;
@@ -756,60 +868,63 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
       const short* col = rt.col + (size_t)at.e * 8 * NT + nt * 8;
       const int p = col[g];
       const long long i = (long long)p * a.I + at.c * K::kChunk + q * K::kVec;
-      o.v[nt][0] = make_uint4(0, 0, 0, 0);
       if constexpr (WT == kBf16) {
-        o.v[nt][1] = o.v[nt][0];
-        if (p >= 0 && in) {
-          o.v[nt][0] = __ldcg(reinterpret_cast<const uint4*>(a.h_hi + i));
-          o.v[nt][1] = __ldcg(reinterpret_cast<const uint4*>(a.h_lo + i));
-        }
+        o.v[nt][0] = load_or_zero(a.h_hi + i, p >= 0 && in);
+        o.v[nt][1] = load_or_zero(a.h_lo + i, p >= 0 && in);
       } else {
-        if (p >= 0 && in) o.v[nt][0] = __ldcg(reinterpret_cast<const uint4*>(a.hq + i));
+        o.v[nt][0] = load_or_zero(a.hq + i, p >= 0 && in);
         const int p0 = col[2 * q], p1 = col[2 * q + 1];
         o.cf[nt][0] = p0 >= 0 ? __ldcg(a.h_scale + p0) : 0.f;
         o.cf[nt][1] = p1 >= 0 ? __ldcg(a.h_scale + p1) : 0.f;
       }
     }
   };
-  for (int row = r0, n; row < r1; row += n) {
-    n = min(16, r1 - row);
+  for (int row = r0; row < r1;) {
     float acc[NT][4] = {};
-    DownCursor at, ahead;
-    at.start(row, r1, C, D);
-    ahead = at;
+    at.start(row);
+    const int n = at.n;
+    DownCursor ahead = at;
     Operand ops[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (ahead.e < D) { fetch(ahead, ops[j]); ahead.next(C, D); }
-    while (at.e < D) {
+      if (ahead.in_tile()) { fetch(ahead, ops[j]); ahead.next(); }
+    while (at.in_tile()) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        if (at.e >= D) break;
+        if (!at.in_tile()) break;
         Operand& now = ops[j];
         uint4 wa, wb;
         fifo.front(&wa, &wb);
-        Wide fa, fb;
-        if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
-        const unsigned mask = rt.mask[at.e];
+        if (LORA && at.e >= D) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (NT > 1 && !(mask >> nt & 1)) continue;
-          if constexpr (WT == kBf16) {
+          for (int nt = 0; nt < NT; ++nt) {
             chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][0]);
-            chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][1]);
-          } else {
-            typename K::Acc part[4] = {};
-            if constexpr (WT == kInt8) chunk_mma_s8(part, wa, wb, now.v[nt][0]);
-            if constexpr (WT == kFp8) chunk_mma_fp8(part, fa, fb, now.v[nt][0]);
-            acc[nt][0] += (float)part[0] * (now.rf[0] * now.cf[nt][0]);
-            acc[nt][1] += (float)part[1] * (now.rf[0] * now.cf[nt][1]);
-            acc[nt][2] += (float)part[2] * (now.rf[1] * now.cf[nt][0]);
-            acc[nt][3] += (float)part[3] * (now.rf[1] * now.cf[nt][1]);
+            chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][LORA]);
+          }
+        } else {
+          Wide fa, fb;
+          if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
+          const unsigned mask = rt.mask[at.e];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (NT > 1 && !(mask >> nt & 1)) continue;
+            if constexpr (WT == kBf16) {
+              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][0]);
+              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][1]);
+            } else {
+              typename K::Acc part[4] = {};
+              if constexpr (WT == kInt8) chunk_mma_s8(part, wa, wb, now.v[nt][0]);
+              if constexpr (WT == kFp8) chunk_mma_fp8(part, fa, fb, now.v[nt][0]);
+              acc[nt][0] += (float)part[0] * (now.rf[0] * now.cf[nt][0]);
+              acc[nt][1] += (float)part[1] * (now.rf[0] * now.cf[nt][1]);
+              acc[nt][2] += (float)part[2] * (now.rf[1] * now.cf[nt][0]);
+              acc[nt][3] += (float)part[3] * (now.rf[1] * now.cf[nt][1]);
+            }
           }
         }
         push();
-        at.next(C, D);
-        if (ahead.e < D) { fetch(ahead, now); ahead.next(C, D); }
+        at.next();
+        if (ahead.in_tile()) { fetch(ahead, now); ahead.next(); }
       }
     }
     float* mine = red + warp * 16 * 8 * NT;
@@ -828,17 +943,10 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) s += red[(k * 16 + i) * 8 * NT + t];
-      if (a.lora.r) {
-        for (int p = t * a.k; p < (t + 1) * a.k; ++p) {
-          long long m;
-          if (rt.pair_slot[p] < 0 || adapter_of(a, p, &m) < 0) continue;
-          s += dot_row(a.lora.b2 + (m * a.H + row + i) * a.lora.r,
-                       a.v + (size_t)p * a.lora.r, a.lora.r);
-        }
-      }
       a.out[t * a.ldo + row + i] = __float2bfloat16(s);
     }
     __syncthreads();
+    row += n;
   }
 }
 
@@ -1016,16 +1124,18 @@ size_t staged_bytes(int T, int H, int wtype) {
 
 int column_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
 
-// Shared memory of up_kernel without the copy of x; down_kernel needs less.
-size_t up_bytes(int P, int NT) {
-  return kFifoBytes + routing_bytes(P, NT) + 2 * (size_t)kWarps * 16 * 8 * NT * 4 +
-         kMaxTokens * 4;
+// Shared memory of up_kernel without the copy of x, and of down_kernel.
+size_t up_bytes(int P, int NT, bool lora) {
+  return kFifoBytes + routing_bytes(P, NT, lora) + kMaxTokens * 4;
+}
+size_t down_bytes(int P, int NT, bool lora) {
+  return kFifoBytes + routing_bytes(P, NT, lora) + (size_t)kWarps * 16 * 8 * NT * 4;
 }
 
 // Does the copy of x fit beside it?  bf16 rows are read from L1 / L2 where it does not.
 bool fits_staged(int T, int k, int H, int wtype) {
   const int NT = column_tiles(T);
-  return up_bytes(T * k, NT) + staged_bytes(T, H, wtype) <= kSmem;
+  return up_bytes(T * k, NT, true) + staged_bytes(T, H, wtype) + kMaxTokens * 4 <= kSmem;
 }
 
 // Tokens of one launch: as many as fit the column tiles, the pair tables and (8-bit
@@ -1057,45 +1167,54 @@ size_t carve(ExpertsArgs* a, unsigned char* base, size_t pairs, int I, int wtype
     a->h_scale = reinterpret_cast<float*>(take(pairs * 4));
   }
   if (r) {
-    a->u = reinterpret_cast<float*>(take(pairs * 2 * r * 4));
-    a->v = reinterpret_cast<float*>(take(pairs * r * 4));
+    a->u_hi = reinterpret_cast<__nv_bfloat16*>(take(pairs * 2 * r * 2));
+    a->u_lo = reinterpret_cast<__nv_bfloat16*>(take(pairs * 2 * r * 2));
+    a->v_hi = reinterpret_cast<__nv_bfloat16*>(take(pairs * r * 2));
+    a->v_lo = reinterpret_cast<__nv_bfloat16*>(take(pairs * r * 2));
   }
   return at;
 }
 
-template <int WT, int NT>
+template <int WT, int NT, bool LORA>
 int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
   static std::atomic<bool> done_up[kMaxDevices], done_down[kMaxDevices];
   int dev = 0, sms = 0;
   int rc = device_sms(&dev, &sms);
   if (rc != 0) return rc;
-  cudaError_t err = allow_smem(up_kernel<WT, NT>, done_up, dev);
-  if (err == cudaSuccess) err = allow_smem(down_kernel<WT, NT>, done_down, dev);
+  cudaError_t err = allow_smem(up_kernel<WT, NT, LORA>, done_up, dev);
+  if (err == cudaSuccess) err = allow_smem(down_kernel<WT, NT, LORA>, done_down, dev);
   if (err != cudaSuccess) return (int)err;
   const int P = a.T * a.k;
-  if (a.lora.r) {
+  if (LORA) {
     rc = launch(shrink_kernel, dim3(P, (2 * a.lora.r + kWarps - 1) / kWarps), kThreads, 0,
                 stream, a);
     if (rc != 0) return rc;
   }
   const int staged = fits_staged(a.T, a.k, a.H, WT);
-  rc = launch(up_kernel<WT, NT>, dim3(sms), kThreads,
-              up_bytes(P, NT) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a, staged);
+  rc = launch(up_kernel<WT, NT, LORA>, dim3(sms), kThreads,
+              up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a,
+              staged);
   if (rc != 0) return rc;
-  if (WT != kBf16 || a.lora.r) {
-    rc = launch(mid_kernel<WT>, dim3(P), kThreads, 0, stream, a);
+  if (WT != kBf16 || LORA) {
+    rc = launch(mid_kernel<WT, LORA>, dim3(P), kThreads, 0, stream, a);
     if (rc != 0) return rc;
   }
-  return launch(down_kernel<WT, NT>, dim3(sms), kThreads, up_bytes(P, NT), stream, a);
+  return launch(down_kernel<WT, NT, LORA>, dim3(sms), kThreads, down_bytes(P, NT, LORA), stream,
+                a);
+}
+
+template <int WT, bool LORA>
+int run_tiles(const ExpertsArgs& a, cudaStream_t stream) {
+  switch (column_tiles(a.T)) {
+    case 1: return run_layer<WT, 1, LORA>(a, stream);
+    case 2: return run_layer<WT, 2, LORA>(a, stream);
+    default: return run_layer<WT, 4, LORA>(a, stream);
+  }
 }
 
 template <int WT>
 int run_type(const ExpertsArgs& a, cudaStream_t stream) {
-  switch (column_tiles(a.T)) {
-    case 1: return run_layer<WT, 1>(a, stream);
-    case 2: return run_layer<WT, 2>(a, stream);
-    default: return run_layer<WT, 4>(a, stream);
-  }
+  return a.lora.r ? run_tiles<WT, true>(a, stream) : run_tiles<WT, false>(a, stream);
 }
 
 bool misaligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
@@ -1201,7 +1320,7 @@ int expert_cache_experts_lora(const void* x, int T, int ldx, int H, const int* i
                               long workspace_bytes, cudaStream_t stream) {
   ExpertsArgs a = experts_args(x, T, ldx, H, ids, weights, k, expert_map, n_map, w13, w13_scale,
                                w2, w2_scale, S, I, out, ldo);
-  if (L <= 0 || E <= 0 || r <= 0 || r > EXPERT_CACHE_LORA_MAX_RANK || r % 8) return -1;
+  if (L <= 0 || E <= 0 || (long long)L * E > INT_MAX || r <= 0 || r > EXPERT_CACHE_LORA_MAX_RANK || r % 8) return -1;
   if (!adapter || !a13 || !b13 || !a2 || !b2 || !scaling) return -1;
   if (misaligned(a13, 16) || misaligned(b13, 16) || misaligned(a2, 16) || misaligned(b2, 16) ||
       misaligned(adapter, 4) || misaligned(scaling, 4))
