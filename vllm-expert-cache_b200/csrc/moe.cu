@@ -248,7 +248,7 @@ struct Kind<kInt8> {
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2,
                                          unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -256,7 +256,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2,
                                         unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -264,7 +264,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1,
 }
 __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2,
                                        unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -313,25 +313,22 @@ __device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, cons
 
 // ---------------------------------------------------------------------------------------
 // The stream of weights.  Every thread copies the very bytes that it will multiply into a
-// FIFO of its own in shared memory (cp.async, two 16-byte vectors a stage), so the stream
-// needs no barrier and no thread waits for another's data; kStages * 8 KB per SM are on
-// their way at any time, several times what the memory's latency asks for, which covers
-// the barriers and the tile ends too.
+// FIFO of its own in shared memory (cp.async), so the stream needs no barrier and no thread
+// waits for another's data.  A stage is a block of KB chunks, that is KB * 64 contiguous
+// bytes of each of the 16 rows: addresses, waits and branches are paid once a block.  (With
+// a stage a chunk the kernels executed 100 to 230 instructions a chunk and were bound by
+// issuing them, at 0.37 of the memory's rate.)  128 KB an SM are on their way at any time,
+// several times what the memory's latency asks for.
 
-constexpr int kStages = 16;
-constexpr int kFifoBytes = kStages * kThreads * 32;
+constexpr int kFifoBytes = 128 * 1024;
 
-__device__ __forceinline__ void copy16(unsigned char* dst, const uint8_t* src, bool in) {
-  const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+__device__ __forceinline__ void copy16(unsigned dst, const uint8_t* src, bool in) {
   const int n = in ? 16 : 0;                   // 0: the vector is zero-filled, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// The oldest of kStages committed stages has landed.
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-}
+
 // 16 bytes from L2, or zeros and no read.
 __device__ __forceinline__ uint4 load_or_zero(const void* p, bool in) {
   uint4 r;
@@ -344,22 +341,40 @@ __device__ __forceinline__ uint4 load_or_zero(const void* p, bool in) {
   return r;
 }
 
+__device__ __forceinline__ uint4 load_shared(unsigned at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(at)
+               : "memory");
+  return r;
+}
+
+template <int KB>
 struct Fifo {
-  unsigned char* base;       // this thread's vectors of stage 0
-  int put, get;
-  __device__ __forceinline__ explicit Fifo(unsigned char* smem)
-      : base(smem + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 16), put(0), get(0) {}
-  __device__ __forceinline__ unsigned char* slot(int i) const { return base + i * (kThreads * 32); }
-  __device__ __forceinline__ void push(const uint8_t* a, bool in_a, const uint8_t* b, bool in_b) {
-    copy16(slot(put), a, in_a);
-    copy16(slot(put) + 512, b, in_b);
-    put = put + 1 == kStages ? 0 : put + 1;
+  static constexpr int kStage = kThreads * KB * 32, kStages = kFifoBytes / kStage;
+  unsigned base, put, get;       // this thread's vectors of stage 0, of the next to fill / read
+  __device__ __forceinline__ explicit Fifo(const void* smem) {
+    base = (unsigned)__cvta_generic_to_shared(smem) + (threadIdx.x >> 5) * (KB * 1024) +
+           (threadIdx.x & 31) * 16;
+    put = get = base;
   }
-  __device__ __forceinline__ void front(uint4* a, uint4* b) {
-    copy_wait();
-    *a = *reinterpret_cast<const uint4*>(slot(get));
-    *b = *reinterpret_cast<const uint4*>(slot(get) + 512);
-    get = get + 1 == kStages ? 0 : get + 1;
+  // The next block of row `a` (row g) and row `b` (row g + 8), `left_*` bytes of them left to
+  // read (nothing is read past them).
+  __device__ __forceinline__ void push(const uint8_t* a, int left_a, const uint8_t* b, int left_b) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      copy16(put + j * 1024, a + j * 64, left_a > j * 64);
+      copy16(put + j * 1024 + 512, b + j * 64, left_b > j * 64);
+    }
+    put = put == base + (kStages - 1) * kStage ? base : put + kStage;
+  }
+  // Waits until the oldest stage has landed; its vectors are at the returned address.
+  __device__ __forceinline__ unsigned front() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    const unsigned at = get;
+    get = get == base + (kStages - 1) * kStage ? base : get + kStage;
+    return at;
   }
 };
 
@@ -385,8 +400,15 @@ __device__ __forceinline__ float clamp_top(unsigned bits) {
   return m < 1e-10f ? 1e-10f : m;
 }
 
-// x of the CTA's tokens in shared memory as [chunk][T][64 bytes] (zeros past H), quantised
-// for 8-bit weights with the scales in `xs`.  Whole CTA; ends with a barrier.
+// Where chunk j of block `blk` of token t lies in the staged x: [block][T][4 chunks], a
+// token's odd and even chunks swapped for odd t, so that eight lanes of two tokens read all
+// banks.
+__device__ __forceinline__ int staged_at(int T, int blk, int t, int j) {
+  return (blk * T + t) * 256 + ((j ^ (t & 1)) * 64);
+}
+
+// x of the CTA's tokens in shared memory (zeros past H), quantised for 8-bit weights with the
+// scales in `xs`.  Whole CTA; ends with a barrier.
 template <int WT>
 __device__ void stage_x(const ExpertsArgs& a, unsigned char* st, float* xs) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -418,7 +440,7 @@ __device__ void stage_x(const ExpertsArgs& a, unsigned char* st, float* xs) {
     if (tid < a.T) xs[tid] = clamp_top(tops[tid]);
     __syncthreads();
   }
-  const int pieces = (a.H + kChunk - 1) / kChunk * 4;        // 16 bytes each, of a token
+  const int pieces = (a.H + 4 * kChunk - 1) / (4 * kChunk) * 16;   // 16 bytes each, of a token
   for (int i = tid; i < pieces * a.T; i += kThreads) {
     const int t = i / pieces, m = i - t * pieces;
     uint4 o = make_uint4(0, 0, 0, 0);
@@ -444,7 +466,7 @@ __device__ void stage_x(const ExpertsArgs& a, unsigned char* st, float* xs) {
         o = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    *reinterpret_cast<uint4*>(st + ((size_t)(m >> 2) * a.T + t) * 64 + (m & 3) * 16) = o;
+    *reinterpret_cast<uint4*>(st + staged_at(a.T, m >> 4, t, m >> 2 & 3) + (m & 3) * 16) = o;
   }
   __syncthreads();
   if (WT != kBf16) {
@@ -515,14 +537,14 @@ struct UpTile {
   }
 };
 
-template <int WT, int NT, bool LORA>
-__global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__ ExpertsArgs a,
-                                                         int staged) {
+template <int WT, int NT, bool LORA, bool STAGED>
+__global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
   using Acc = typename K::Acc;
+  constexpr int KB = 4;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  Fifo fifo(smem);
+  Fifo<KB> fifo(smem);
   const Routing rt = routing_at(smem + kFifoBytes, P, NT);
   float* xs = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT, LORA));
   unsigned char* st = reinterpret_cast<unsigned char*>(xs + kMaxTokens);
@@ -537,38 +559,44 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   const long long R = (long long)D * a.I, W = (long long)gridDim.x * kWarps;
   const int w = blockIdx.x * kWarps + warp;
   const int r0 = (int)(R * w / W), r1 = (int)(R * (w + 1) / W);
-  const int C = (a.H + K::kChunk - 1) / K::kChunk;
-  const int RC = LORA ? (a.lora.r + 31) / 32 : 0;
-  const long long row_bytes = (long long)a.H * K::kItem;
+  const int row_bytes = a.H * K::kItem, lora_bytes = LORA ? a.lora.r * 2 : 0;
+  const long long up_off = (long long)a.I * row_bytes;
 
-  // The chunks of the warp's tiles in order, each tile's adapted columns after them; `src`
-  // and the counters follow the head of the stream.
+  // The blocks of the warp's tiles in order, those of each tile's adapted columns after them;
+  // `src` and the counters follow the head of the stream.
   UpTile head;
   const uint8_t* src = nullptr;
-  int hc = 0, hr = 0;
-  unsigned left = 0;
+  int pos = 0;                  // bytes of the row (of B13's, past the row's end) gone by
+  unsigned adapted = 0;
   const auto head_at = [&](int row) {
     head.at(row, r1, a.I);
     src = a.w13 + ((long long)rt.slot[head.e] * 2 * a.I + head.i0 + g) * row_bytes + q * 16;
-    hc = 0;
-    if (LORA) left = rt.adapted[head.e];
+    pos = 0;
+    if (LORA) adapted = rt.adapted[head.e];
   };
   const auto push = [&]() {
     if (head.row < r1) {
-      if (hc < C) {
-        const bool in = g < head.n && hc * K::kChunk + q * K::kVec < a.H;
-        fifo.push(src + hc * 64, in, src + a.I * row_bytes + hc * 64, in);
-        ++hc;
-      } else if (LORA) {
-        const int p = rt.col[(size_t)head.e * 8 * NT + __ffs(left) - 1];
-        const bool in = g < head.n && hr * 32 + q * 8 < a.lora.r;
-        const __nv_bfloat16* b = a.lora.b13 + ((long long)rt.matrix[p] * 2 * a.I + head.i0 + g) *
-                                                  a.lora.r + hr * 32 + q * 8;
-        fifo.push(reinterpret_cast<const uint8_t*>(b), in,
-                  reinterpret_cast<const uint8_t*>(b + (long long)a.I * a.lora.r), in);
-        if (++hr == RC) { hr = 0; left &= left - 1; }
+      const bool mine = g < head.n;
+      if (!LORA || pos < row_bytes) {
+        const int left = mine ? row_bytes - pos - q * 16 : 0;
+        fifo.push(src, left, src + up_off, left);
+        src += KB * 64;
+        pos += KB * 64;
+      } else {
+        const int at = pos - (row_bytes + KB * 64 - 1) / (KB * 64) * (KB * 64);
+        const int p = rt.col[(size_t)head.e * 8 * NT + __ffs(adapted) - 1];
+        const uint8_t* b = reinterpret_cast<const uint8_t*>(a.lora.b13) +
+                           ((long long)rt.matrix[p] * 2 * a.I + head.i0 + g) * lora_bytes + at +
+                           q * 16;
+        const int left = mine ? lora_bytes - at - q * 16 : 0;
+        fifo.push(b, left, b + (long long)a.I * lora_bytes, left);
+        pos += KB * 64;
+        if (at + KB * 64 >= lora_bytes) {
+          pos -= at + KB * 64;
+          adapted &= adapted - 1;
+        }
       }
-      if (hc >= C && (!LORA || left == 0)) {
+      if (pos >= row_bytes && (!LORA || adapted == 0)) {
         const int next = head.row + head.n;
         if (next < r1) head_at(next);
         else head.row = r1;
@@ -578,10 +606,22 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   };
   head.row = r1;
   if (r0 < r1) head_at(r0);
-  for (int i = 0; i < kStages; ++i) push();
+  for (int i = 0; i < Fifo<KB>::kStages; ++i) push();
 
-  if (staged) stage_x<WT>(a, st, xs);
+  if (STAGED) stage_x<WT>(a, st, xs);
   if (LORA) grid_dependency_wait();
+
+  // Column g's token of each column tile.  Past the last token: any (the column is not kept).
+  unsigned xa[NT], xb[NT];                      // staged: even and odd chunks
+  const __nv_bfloat16* xg[NT];                  // not staged: the row in global memory
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int t = min(nt * 8 + g, a.T - 1);
+    const unsigned at = (unsigned)__cvta_generic_to_shared(st) + q * 16;
+    xa[nt] = at + staged_at(a.T, 0, t, 0);
+    xb[nt] = at + staged_at(a.T, 0, t, 1);
+    xg[nt] = a.x + t * a.ldx + q * 8;
+  }
 
   UpTile tile;
   for (int row = r0; row < r1; row += tile.n) {
@@ -596,27 +636,33 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       su = a.s13[(long long)slot * 2 * a.I + a.I + r];
     }
     Acc acc[NT][4] = {};
-#pragma unroll 2
-    for (int c = 0; c < C; ++c) {
-      uint4 wa, wb;
-      fifo.front(&wa, &wb);
-      Wide fa, fb;
-      if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
-      const bool in = c * K::kChunk + q * K::kVec < a.H;
+    for (int at = 0, blk = 0; at < row_bytes; at += KB * 64, blk += a.T * 256) {
+      const unsigned f = fifo.front();
+      uint4 wa[KB], wb[KB];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (NT > 1 && !(mask >> nt & 1)) continue;
-        const int t = nt * 8 + g;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (t < a.T) {
-          if (staged)
-            v = *reinterpret_cast<const uint4*>(st + ((size_t)c * a.T + t) * 64 + q * 16);
-          else if (in)
-            v = *reinterpret_cast<const uint4*>(a.x + t * a.ldx + c * K::kChunk + q * K::kVec);
+      for (int j = 0; j < KB; ++j) {
+        wa[j] = load_shared(f + j * 1024);
+        wb[j] = load_shared(f + j * 1024 + 512);
+      }
+#pragma unroll
+      for (int j = 0; j < KB; ++j) {
+        Wide fa, fb;
+        if (WT == kFp8) { fa = widen(wa[j]); fb = widen(wb[j]); }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (NT > 1 && !(mask >> nt & 1)) continue;
+          uint4 v;
+          if constexpr (STAGED) {
+            v = load_shared((j & 1 ? xb[nt] : xa[nt]) + blk + (j & 2) * 64);
+          } else {
+            v = make_uint4(0, 0, 0, 0);
+            if (at + j * 64 + q * 16 < row_bytes)
+              v = *reinterpret_cast<const uint4*>(xg[nt] + (at + j * 64) / 2);
+          }
+          if constexpr (WT == kBf16) chunk_mma_bf16(acc[nt], wa[j], wb[j], v);
+          if constexpr (WT == kInt8) chunk_mma_s8(acc[nt], wa[j], wb[j], v);
+          if constexpr (WT == kFp8) chunk_mma_fp8(acc[nt], fa, fb, v);
         }
-        if constexpr (WT == kBf16) chunk_mma_bf16(acc[nt], wa, wb, v);
-        if constexpr (WT == kInt8) chunk_mma_s8(acc[nt], wa, wb, v);
-        if constexpr (WT == kFp8) chunk_mma_fp8(acc[nt], fa, fb, v);
       }
       push();      // into the stage just read, whose vectors the products have taken
     }
@@ -627,24 +673,28 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       const uint4 zero = make_uint4(0, 0, 0, 0);
       for (unsigned cols = rt.adapted[tile.e]; cols; cols &= cols - 1) {
         const int t = __ffs(cols) - 1;
-        const size_t at = (size_t)col[t] * 2 * a.lora.r + q * 8;
-        for (int rc = 0; rc < RC; ++rc) {
-          const bool has = g == (t & 7) && rc * 32 + q * 8 < a.lora.r;
-          const uint4 v[4] = {load_or_zero(a.u_hi + at + rc * 32, has),
-                              load_or_zero(a.u_lo + at + rc * 32, has),
-                              load_or_zero(a.u_hi + at + a.lora.r + rc * 32, has),
-                              load_or_zero(a.u_lo + at + a.lora.r + rc * 32, has)};
-          uint4 wa, wb;
-          fifo.front(&wa, &wb);
+        const size_t up = (size_t)col[t] * 2 * a.lora.r + q * 8;
+        for (int at = 0; at < lora_bytes; at += KB * 64) {
+          const unsigned f = fifo.front();
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            // (a product with zeros in the other column tiles: a branch around it would
-            // index the accumulators at run time and put them into local memory)
-            const bool here = NT == 1 || t >> 3 == nt;
-            chunk_mma_bf16(add[nt], wa, zero, here ? v[0] : zero);
-            chunk_mma_bf16(add[nt], wa, zero, here ? v[1] : zero);
-            chunk_mma_bf16(add[nt], zero, wb, here ? v[2] : zero);
-            chunk_mma_bf16(add[nt], zero, wb, here ? v[3] : zero);
+          for (int j = 0; j < KB; ++j) {
+            if (at + j * 64 >= lora_bytes) break;
+            const bool has = g == (t & 7) && at + j * 64 + q * 16 < lora_bytes;
+            const size_t i = up + at / 2 + j * 32;
+            const uint4 v[4] = {load_or_zero(a.u_hi + i, has), load_or_zero(a.u_lo + i, has),
+                                load_or_zero(a.u_hi + i + a.lora.r, has),
+                                load_or_zero(a.u_lo + i + a.lora.r, has)};
+            const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              // (a product with zeros in the other column tiles: a branch around it would
+              // index the accumulators at run time and put them into local memory)
+              const bool here = NT == 1 || t >> 3 == nt;
+              chunk_mma_bf16(add[nt], wa, zero, here ? v[0] : zero);
+              chunk_mma_bf16(add[nt], wa, zero, here ? v[1] : zero);
+              chunk_mma_bf16(add[nt], zero, wb, here ? v[2] : zero);
+              chunk_mma_bf16(add[nt], zero, wb, here ? v[3] : zero);
+            }
           }
           push();
         }
@@ -746,11 +796,11 @@ __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ E
 // down
 
 // Where a warp is in the stream of a CTA's rows: a tile of up to 16 rows after the other, in
-// each the C chunks of every entry and then, as entries from D on, the RC chunks of every
-// adapted pair; the warps take these chunks in turn.
+// each the CB blocks of every entry and then, as entries from D on, the RB blocks of every
+// adapted pair; the warps take these blocks in turn.
 struct DownCursor {
   int row, n, e, c;
-  int r1, C, D, RC, N;       // N = entries + adapted pairs
+  int r1, CB, D, RB, N;       // N = entries + adapted pairs
   __device__ __forceinline__ void start(int r) {
     row = r;
     const int left = r1 - r, tiles = (left + 15) / 16;
@@ -760,7 +810,7 @@ struct DownCursor {
     wrap();
   }
   __device__ __forceinline__ void wrap() {
-    while (e < N && c >= (e < D ? C : RC)) { c -= e < D ? C : RC; ++e; }
+    while (e < N && c >= (e < D ? CB : RB)) { c -= e < D ? CB : RB; ++e; }
   }
   __device__ __forceinline__ bool in_tile() const { return e < N; }
   // On to the next tile where this one is done; false after the last.
@@ -777,10 +827,17 @@ struct DownCursor {
   }
 };
 
-// The other operand of a chunk, in registers: read from L2 kAhead chunks ahead.
+// Chunks per block: the other operand of two blocks has to fit the registers.
+template <int WT, int NT>
+constexpr int kDownBlock = WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
+
+// The other operand of a block, read from L2 while the block before it is multiplied.
 template <int WT, int NT, bool LORA>
 struct DownOperand {
-  uint4 v[NT][WT == kBf16 || LORA ? 2 : 1];
+  static constexpr int KB = kDownBlock<WT, NT>;
+  // of an adapter's block: chunks (their hi and lo parts take two vectors each)
+  static constexpr int LB = WT == kBf16 ? KB : KB / 2;
+  uint4 v[NT][WT == kBf16 ? 2 * KB : KB];
   float rf[2], cf[NT][2];       // 8-bit: scales of rows g, g + 8 and of columns 2q, 2q + 1
 };
 
@@ -790,9 +847,11 @@ constexpr int kRed = kWarps * 16 * 8 * NT;   // the warps' partial sums
 template <int WT, int NT, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
+  using Operand = DownOperand<WT, NT, LORA>;
+  constexpr int KB = Operand::KB, LB = Operand::LB;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  Fifo fifo(smem);
+  Fifo<KB> fifo(smem);
   const Routing rt = routing_at(smem + kFifoBytes, P, NT);
   float* red = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT, LORA));
 
@@ -806,56 +865,56 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
   const int D = rt.entries[0];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const long long row_bytes = (long long)a.I * K::kItem;
+  const int row_bytes = a.I * K::kItem, lora_bytes = LORA ? a.lora.r * 2 : 0;
 
   DownCursor head;
   head.r1 = r1;
-  head.C = (a.I + K::kChunk - 1) / K::kChunk;
+  head.CB = (row_bytes + KB * 64 - 1) / (KB * 64);
   head.D = D;
-  head.RC = LORA ? (a.lora.r + 31) / 32 : 1;
+  head.RB = LORA ? (lora_bytes + LB * 64 - 1) / (LB * 64) : 1;
   head.N = D + (LORA ? rt.entries[2] : 0);
   bool more = r0 < r1 && head.N > 0;
   head.start(r0);
   const auto push = [&]() {
     if (more && (more = head.settle())) {
+      const uint8_t* src;
+      int left, stride;
       if (!LORA || head.e < D) {
-        const bool in = head.c * K::kChunk + q * K::kVec < a.I;
-        const uint8_t* src =
-            a.w2 + ((long long)rt.slot[head.e] * a.H + head.row + g) * row_bytes + head.c * 64 +
-            q * 16;
-        fifo.push(src, in && g < head.n, src + 8 * row_bytes, in && g + 8 < head.n);
+        const int at = head.c * (KB * 64) + q * 16;
+        src = a.w2 + ((long long)rt.slot[head.e] * a.H + head.row + g) * row_bytes + at;
+        left = row_bytes - at;
+        stride = row_bytes;
       } else {
-        const int p = rt.list[head.e - D];
-        const bool in = head.c * 32 + q * 8 < a.lora.r;
-        const __nv_bfloat16* b = a.lora.b2 + ((long long)rt.matrix[p] * a.H + head.row + g) *
-                                                 a.lora.r + head.c * 32 + q * 8;
-        fifo.push(reinterpret_cast<const uint8_t*>(b), in && g < head.n,
-                  reinterpret_cast<const uint8_t*>(b + 8 * a.lora.r), in && g + 8 < head.n);
+        const int at = head.c * (LB * 64) + q * 16;
+        src = reinterpret_cast<const uint8_t*>(a.lora.b2) +
+              ((long long)rt.matrix[rt.list[head.e - D]] * a.H + head.row + g) * lora_bytes + at;
+        left = min(lora_bytes - at, LB * 64);
+        stride = lora_bytes;
       }
+      fifo.push(src, g < head.n ? left : 0, src + 8LL * stride, g + 8 < head.n ? left : 0);
       head.next();
     }
     copy_commit();
   };
   DownCursor at = head;
-  for (int i = 0; i < kStages; ++i) push();
+  for (int i = 0; i < Fifo<KB>::kStages; ++i) push();
 
   grid_dependency_wait();
-  using Operand = DownOperand<WT, NT, LORA>;
-  constexpr int kAhead = NT == 4 ? 2 : 4;
   const auto fetch = [&](const DownCursor& at, Operand& o) {
     if (LORA && at.e >= D) {
-      const int p = rt.list[at.e - D], t = p / a.k;
-      const size_t i = (size_t)p * a.lora.r + at.c * 32 + q * 8;
-      const bool in = g == (t & 7) && at.c * 32 + q * 8 < a.lora.r;
+      const int p = rt.list[at.e - D], t = p / a.k, pos = at.c * (LB * 64) + q * 16;
+      const size_t i = (size_t)p * a.lora.r + pos / 2;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const bool here = in && (NT == 1 || t >> 3 == nt);
-        o.v[nt][0] = load_or_zero(a.v_hi + i, here);
-        o.v[nt][LORA] = load_or_zero(a.v_lo + i, here);
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < LB; ++j) {
+          const bool here = (NT == 1 || t >> 3 == nt) && g == (t & 7) && pos + j * 64 < lora_bytes;
+          o.v[nt][2 * j] = load_or_zero(a.v_hi + i + j * 32, here);
+          o.v[nt][2 * j + 1] = load_or_zero(a.v_lo + i + j * 32, here);
+        }
       return;
     }
-    const bool in = at.c * K::kChunk + q * K::kVec < a.I;
+    const int pos = at.c * (KB * 64) + q * 16;
     if (WT != kBf16) {
       const float* s2 = a.s2 + (long long)rt.slot[at.e] * a.H + at.row;
       o.rf[0] = g < at.n ? s2[g] : 0.f;
@@ -867,12 +926,18 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
       if (NT > 1 && !(mask >> nt & 1)) continue;
       const short* col = rt.col + (size_t)at.e * 8 * NT + nt * 8;
       const int p = col[g];
-      const long long i = (long long)p * a.I + at.c * K::kChunk + q * K::kVec;
-      if constexpr (WT == kBf16) {
-        o.v[nt][0] = load_or_zero(a.h_hi + i, p >= 0 && in);
-        o.v[nt][1] = load_or_zero(a.h_lo + i, p >= 0 && in);
-      } else {
-        o.v[nt][0] = load_or_zero(a.hq + i, p >= 0 && in);
+      const int left = p >= 0 ? row_bytes - pos : 0;
+      const long long i = (long long)p * row_bytes + pos;
+#pragma unroll
+      for (int j = 0; j < KB; ++j) {
+        if constexpr (WT == kBf16) {
+          o.v[nt][2 * j] = load_or_zero(reinterpret_cast<const uint8_t*>(a.h_hi) + i + j * 64, left > j * 64);
+          o.v[nt][2 * j + 1] = load_or_zero(reinterpret_cast<const uint8_t*>(a.h_lo) + i + j * 64, left > j * 64);
+        } else {
+          o.v[nt][j] = load_or_zero(a.hq + i + j * 64, left > j * 64);
+        }
+      }
+      if (WT != kBf16) {
         const int p0 = col[2 * q], p1 = col[2 * q + 1];
         o.cf[nt][0] = p0 >= 0 ? __ldcg(a.h_scale + p0) : 0.f;
         o.cf[nt][1] = p1 >= 0 ? __ldcg(a.h_scale + p1) : 0.f;
@@ -884,41 +949,58 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
     at.start(row);
     const int n = at.n;
     DownCursor ahead = at;
-    Operand ops[kAhead];
+    Operand ops[2];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (ahead.in_tile()) { fetch(ahead, ops[j]); ahead.next(); }
+    for (int b = 0; b < 2; ++b)
+      if (ahead.in_tile()) { fetch(ahead, ops[b]); ahead.next(); }
     while (at.in_tile()) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
+      for (int b = 0; b < 2; ++b) {
         if (!at.in_tile()) break;
-        Operand& now = ops[j];
-        uint4 wa, wb;
-        fifo.front(&wa, &wb);
+        Operand& now = ops[b];
+        const unsigned f = fifo.front();
         if (LORA && at.e >= D) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][0]);
-            chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][LORA]);
+          for (int j = 0; j < LB; ++j) {
+            const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][2 * j]);
+              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][2 * j + 1]);
+            }
           }
         } else {
-          Wide fa, fb;
-          if (WT == kFp8) { fa = widen(wa); fb = widen(wb); }
           const unsigned mask = rt.mask[at.e];
+          typename K::Acc part[NT][4] = {};
+          uint4 wa[KB], wb[KB];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (NT > 1 && !(mask >> nt & 1)) continue;
-            if constexpr (WT == kBf16) {
-              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][0]);
-              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][1]);
-            } else {
-              typename K::Acc part[4] = {};
-              if constexpr (WT == kInt8) chunk_mma_s8(part, wa, wb, now.v[nt][0]);
-              if constexpr (WT == kFp8) chunk_mma_fp8(part, fa, fb, now.v[nt][0]);
-              acc[nt][0] += (float)part[0] * (now.rf[0] * now.cf[nt][0]);
-              acc[nt][1] += (float)part[1] * (now.rf[0] * now.cf[nt][1]);
-              acc[nt][2] += (float)part[2] * (now.rf[1] * now.cf[nt][0]);
-              acc[nt][3] += (float)part[3] * (now.rf[1] * now.cf[nt][1]);
+          for (int j = 0; j < KB; ++j) {
+            wa[j] = load_shared(f + j * 1024);
+            wb[j] = load_shared(f + j * 1024 + 512);
+          }
+#pragma unroll
+          for (int j = 0; j < KB; ++j) {
+            Wide fa, fb;
+            if (WT == kFp8) { fa = widen(wa[j]); fb = widen(wb[j]); }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (NT > 1 && !(mask >> nt & 1)) continue;
+              if constexpr (WT == kBf16) {
+                chunk_mma_bf16(acc[nt], wa[j], wb[j], now.v[nt][2 * j]);
+                chunk_mma_bf16(acc[nt], wa[j], wb[j], now.v[nt][2 * j + 1]);
+              }
+              if constexpr (WT == kInt8) chunk_mma_s8(part[nt], wa[j], wb[j], now.v[nt][j]);
+              if constexpr (WT == kFp8) chunk_mma_fp8(part[nt], fa, fb, now.v[nt][j]);
+            }
+          }
+          if (WT != kBf16) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (NT > 1 && !(mask >> nt & 1)) continue;
+              acc[nt][0] += (float)part[nt][0] * (now.rf[0] * now.cf[nt][0]);
+              acc[nt][1] += (float)part[nt][1] * (now.rf[0] * now.cf[nt][1]);
+              acc[nt][2] += (float)part[nt][2] * (now.rf[1] * now.cf[nt][0]);
+              acc[nt][3] += (float)part[nt][3] * (now.rf[1] * now.cf[nt][1]);
             }
           }
         }
@@ -1118,8 +1200,8 @@ int launch(void (*fn)(Params...), dim3 grid, int threads, size_t smem, cudaStrea
 int chunk_columns(int wtype) { return wtype == kBf16 ? 32 : 64; }
 
 size_t staged_bytes(int T, int H, int wtype) {
-  const int cc = chunk_columns(wtype);
-  return (size_t)((H + cc - 1) / cc) * 64 * T;
+  const int cc = 4 * chunk_columns(wtype);
+  return (size_t)((H + cc - 1) / cc) * 256 * T;
 }
 
 int column_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
@@ -1177,11 +1259,14 @@ size_t carve(ExpertsArgs* a, unsigned char* base, size_t pairs, int I, int wtype
 
 template <int WT, int NT, bool LORA>
 int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
-  static std::atomic<bool> done_up[kMaxDevices], done_down[kMaxDevices];
+  static std::atomic<bool> done_up[2][kMaxDevices], done_down[kMaxDevices];
   int dev = 0, sms = 0;
   int rc = device_sms(&dev, &sms);
   if (rc != 0) return rc;
-  cudaError_t err = allow_smem(up_kernel<WT, NT, LORA>, done_up, dev);
+  // only bf16 rows may be read where they are
+  const bool staged = WT != kBf16 || fits_staged(a.T, a.k, a.H, WT);
+  const auto up = staged ? up_kernel<WT, NT, LORA, true> : up_kernel<WT, NT, LORA, WT != kBf16>;
+  cudaError_t err = allow_smem(up, done_up[staged], dev);
   if (err == cudaSuccess) err = allow_smem(down_kernel<WT, NT, LORA>, done_down, dev);
   if (err != cudaSuccess) return (int)err;
   const int P = a.T * a.k;
@@ -1190,10 +1275,8 @@ int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
                 stream, a);
     if (rc != 0) return rc;
   }
-  const int staged = fits_staged(a.T, a.k, a.H, WT);
-  rc = launch(up_kernel<WT, NT, LORA>, dim3(sms), kThreads,
-              up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a,
-              staged);
+  rc = launch(up, dim3(sms), kThreads,
+              up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a);
   if (rc != 0) return rc;
   if (WT != kBf16 || LORA) {
     rc = launch(mid_kernel<WT, LORA>, dim3(P), kThreads, 0, stream, a);
