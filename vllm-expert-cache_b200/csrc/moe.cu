@@ -78,6 +78,9 @@ struct ExpertsArgs {
   float* h;                        // 8-bit weights: h [P][I]
   uint8_t* hq;                     // 8-bit weights: quantised h [P][I]
   float* h_scale;                  // 8-bit weights: its scale x weights[t,j] [P]
+  uint8_t* xq;                     // 8-bit weights: quantised x [T][H] where prep_kernel runs
+  float* x_scale;                  // and its scales [T]
+  int prepared;                    // prep_kernel quantises x
   __nv_bfloat16 *u_hi, *u_lo;      // adapters: c A13 x in two parts [P][2r]
   __nv_bfloat16 *v_hi, *v_lo;      // adapters: c weights[t,j] A2 h in two parts [P][r]
   Adapters lora;
@@ -123,6 +126,10 @@ __device__ __forceinline__ Routing routing_at(unsigned char* base, int P, int NT
   return r;
 }
 
+// A map of up to this many entries is copied to shared memory while the ids arrive, so that
+// the two reads do not wait for each other (each may be a miss to DRAM, 0.9 us).
+constexpr int kMapCopy = 1024;
+
 __device__ __forceinline__ int slot_of(const ExpertsArgs& a, int p) {
   int s = a.ids[p];
   if (a.map) s = (s >= 0 && s < a.n_map) ? a.map[s] : -1;
@@ -137,16 +144,29 @@ __device__ __forceinline__ int matrix_of(const ExpertsArgs& a, int p) {
 
 // Whole CTA; ends with a barrier.  Entries are in ascending slot order (repetitions after
 // them in pair order), so sums over entries have one order.
+// `scratch`: kMapCopy ints that nothing else uses yet.
 template <int NT, bool LORA>
-__device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
-  const int P = a.T * a.k, tid = threadIdx.x;
+__device__ void build_routing(const ExpertsArgs& a, const Routing& r, int* scratch) {
+  const int P = a.T * a.k, tid = threadIdx.x, lane = tid & 31;
   constexpr int kWords = kMaxPairs / 32;
+  static_assert(kWords == 32, "a lane holds a word of the slots' bits");
   if (tid < kWords) r.bits[tid] = 0;
   if (tid == 0) r.entries[1] = r.entries[2] = 0;
   for (int i = tid; i < P * 8 * NT / 2; i += kThreads)
     reinterpret_cast<int*>(r.col)[i] = -1;
+  const bool copied = a.map && a.n_map <= kMapCopy;
+  if (copied) {
+#pragma unroll
+    for (int j = 0; j < kMapCopy; j += kThreads)
+      if (tid + j < a.n_map) scratch[tid + j] = a.map[tid + j];
+  }
+  int id = tid < P ? a.ids[tid] : -1;           // (in flight together with the map)
+  if (copied) __syncthreads();
   for (int p = tid; p < P; p += kThreads) {
-    r.pair_slot[p] = (short)slot_of(a, p);
+    if (p != tid) id = a.ids[p];
+    int s = id;
+    if (a.map) s = (id >= 0 && id < a.n_map) ? (copied ? scratch : a.map)[id] : -1;
+    r.pair_slot[p] = (short)(s >= 0 && s < a.S ? s : -1);
     r.mask[p] = 0;
     if (LORA) {
       r.matrix[p] = matrix_of(a, p);
@@ -154,75 +174,68 @@ __device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
     }
   }
   __syncthreads();
-  bool again = false;
   for (int p = tid; p < P; p += kThreads) {
     const int s = r.pair_slot[p];
     if (s < 0) continue;
+    bool again = false;
     for (int q = p - p % a.k; q < p; ++q) again |= r.pair_slot[q] == s;
+    if (again) r.entries[1] = 1;
     atomicOr(&r.bits[s >> 5], 1u << (s & 31));
-  }
-  if (again) r.entries[1] = 1;
-  __syncthreads();
-  if (tid < 32) {
-    const int n = __popc(r.bits[tid]);
-    int sum = n;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, sum, off);
-      if (tid >= off) sum += o;
-    }
-    r.base[tid] = sum - n;
-    if (tid == 31) r.entries[0] = sum;
   }
   __syncthreads();
   const bool repeats = r.entries[1] != 0;
-  for (int p = tid; p < P; p += kThreads) {
-    const int s = r.pair_slot[p];
-    if (s < 0) continue;
-    bool first = true;
-    if (repeats)
+  const unsigned bits = r.bits[lane];           // every warp counts the entries before a word
+  int before = __popc(bits);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += o;
+  }
+  if (tid == 31) r.entries[0] = before;
+  before -= __popc(bits);
+  for (int p0 = tid - lane; p0 < P; p0 += kThreads) {
+    const int p = p0 + lane, s = p < P ? r.pair_slot[p] : -1;
+    const int word = s >= 0 ? s >> 5 : 0;
+    const int base = __shfl_sync(0xffffffffu, before, word);
+    const unsigned b = __shfl_sync(0xffffffffu, bits, word);
+    bool first = s >= 0;
+    if (repeats && s >= 0)
       for (int q = p - p % a.k; q < p; ++q) first &= r.pair_slot[q] != s;
     if (!first) continue;
-    const int e = r.base[s >> 5] + __popc(r.bits[s >> 5] & ((1u << (s & 31)) - 1u));
-    const int t = p / a.k;
+    const int e = base + __popc(b & ((1u << (s & 31)) - 1u)), t = p / a.k;
     r.slot[e] = (short)s;
     r.col[(size_t)e * 8 * NT + t] = (short)p;
+    if (NT == 1) r.mask[e] = 1;
+    else atomicOr(reinterpret_cast<unsigned*>(r.mask) + (e >> 2), 1u << (8 * (e & 3) + (t >> 3)));
     if (LORA && r.matrix[p] >= 0) atomicOr(&r.adapted[e], 1u << t);
   }
+  if (LORA && tid >= kThreads - 32) {      // the adapted pairs in ascending order
+    int n = 0;
+    for (int at = 0; at < P; at += 32) {
+      const int p = at + lane;
+      const bool has = p < P && r.pair_slot[p] >= 0 && r.matrix[p] >= 0;
+      const unsigned b = __ballot_sync(0xffffffffu, has);
+      if (has) r.list[n + __popc(b & ((1u << lane) - 1u))] = (short)p;
+      n += __popc(b);
+    }
+    if (lane == 0) r.entries[2] = n;
+  }
   __syncthreads();
-  if (repeats && tid == 0) {
+  if (!repeats) return;
+  if (tid == 0) {
     int n = r.entries[0];
     for (int p = 0; p < P; ++p) {
-      const int s = r.pair_slot[p];
+      const int s = r.pair_slot[p], t = p / a.k;
       bool first = true;
       for (int q = p - p % a.k; q < p; ++q) first &= r.pair_slot[q] != s;
       if (s < 0 || first) continue;
       r.slot[n] = (short)s;
-      r.col[(size_t)n * 8 * NT + p / a.k] = (short)p;
-      if (LORA && r.matrix[p] >= 0) r.adapted[n] = 1u << p / a.k;
+      r.col[(size_t)n * 8 * NT + t] = (short)p;
+      r.mask[n] = (unsigned char)(1u << (t >> 3));
+      if (LORA && r.matrix[p] >= 0) r.adapted[n] = 1u << t;
       ++n;
     }
     r.entries[0] = n;
-  }
-  if (LORA && tid < 32) {      // the adapted pairs in ascending order
-    int n = 0;
-    for (int at = 0; at < P; at += 32) {
-      const int p = at + tid;
-      const bool has = p < P && r.pair_slot[p] >= 0 && r.matrix[p] >= 0;
-      const unsigned b = __ballot_sync(0xffffffffu, has);
-      if (has) r.list[n + __popc(b & ((1u << tid) - 1u))] = (short)p;
-      n += __popc(b);
-    }
-    if (tid == 0) r.entries[2] = n;
-  }
-  if (repeats) __syncthreads();
-  const int D = r.entries[0];
-  for (int i = tid; i < D * NT; i += kThreads) {
-    const int e = i / NT, nt = i - e * NT;
-    const uint4 c = reinterpret_cast<const uint4*>(r.col)[i];
-    const bool any = (c.x & c.y & c.z & c.w) != 0xffffffffu;
-    if (NT == 1) r.mask[e] = any;
-    else if (any) atomicOr(reinterpret_cast<unsigned*>(r.mask) + (e >> 2), 1u << (8 * (e & 3) + nt));
   }
   __syncthreads();
 }
@@ -236,19 +249,17 @@ __device__ void build_routing(const ExpertsArgs& a, const Routing& r) {
 template <int WT>
 struct Kind {
   static constexpr int kItem = WT == kBf16 ? 2 : 1;      // bytes per weight
-  static constexpr int kVec = 16 / kItem;                // weights per 16 bytes
-  static constexpr int kChunk = 4 * kVec;                // columns per chunk
   using Acc = float;
 };
 template <>
 struct Kind<kInt8> {
-  static constexpr int kItem = 1, kVec = 16, kChunk = 64;
+  static constexpr int kItem = 1;
   using Acc = int;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2,
                                          unsigned a3, unsigned b0, unsigned b1) {
-  asm(
+  asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -256,7 +267,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2,
                                         unsigned a3, unsigned b0, unsigned b1) {
-  asm(
+  asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -264,7 +275,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1,
 }
 __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2,
                                        unsigned a3, unsigned b0, unsigned b1) {
-  asm(
+  asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -317,17 +328,38 @@ __device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, cons
 // waits for another's data.  A stage is a block of KB chunks, that is KB * 64 contiguous
 // bytes of each of the 16 rows: addresses, waits and branches are paid once a block.  (With
 // a stage a chunk the kernels executed 100 to 230 instructions a chunk and were bound by
-// issuing them, at 0.37 of the memory's rate.)  128 KB an SM are on their way at any time,
-// several times what the memory's latency asks for.
+// issuing them, at 0.37 of the memory's rate.)  The FIFOs leave room for a CTA of up and one
+// of down on an SM, so that down has its tables and its first stages before up is done.
 
-constexpr int kFifoBytes = 128 * 1024;
+#ifndef UPKB
+#define UPKB 4
+#endif
+#ifndef UPST
+#define UPST 3
+#endif
+#ifndef DNST
+#define DNST 12
+#endif
+constexpr int kUpBlock = UPKB, kUpStages = UPST;
+constexpr int kUpFifo = kUpStages * kUpBlock * kThreads * 32;
+constexpr int kDownChunks = DNST;              // chunks of a thread's FIFO in down
+constexpr int kDownFifo = kDownChunks * kThreads * 32;
 
-__device__ __forceinline__ void copy16(unsigned dst, const uint8_t* src, bool in) {
-  const int n = in ? 16 : 0;                   // 0: the vector is zero-filled, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+// size 0: the vector is zero-filled and nothing is read.
+__device__ __forceinline__ void copy16_sized(unsigned dst, const uint8_t* src, int size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
                : "memory");
 }
+__device__ __forceinline__ void copy16(unsigned dst, const uint8_t* src, bool in) {
+  copy16_sized(dst, src, in ? 16 : 0);
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// All but the newest N groups of copies have landed.
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // 16 bytes from L2, or zeros and no read.
 __device__ __forceinline__ uint4 load_or_zero(const void* p, bool in) {
@@ -350,9 +382,9 @@ __device__ __forceinline__ uint4 load_shared(unsigned at) {
   return r;
 }
 
-template <int KB>
+template <int KB, int ST>
 struct Fifo {
-  static constexpr int kStage = kThreads * KB * 32, kStages = kFifoBytes / kStage;
+  static constexpr int kStage = kThreads * KB * 32, kStages = ST;
   unsigned base, put, get;       // this thread's vectors of stage 0, of the next to fill / read
   __device__ __forceinline__ explicit Fifo(const void* smem) {
     base = (unsigned)__cvta_generic_to_shared(smem) + (threadIdx.x >> 5) * (KB * 1024) +
@@ -369,9 +401,19 @@ struct Fifo {
     }
     put = put == base + (kStages - 1) * kStage ? base : put + kStage;
   }
+  // The same where the whole block lies in the row; `size_*` 16, or 0 for zeros.
+  __device__ __forceinline__ void push_whole(const uint8_t* a, int size_a, const uint8_t* b,
+                                             int size_b) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      copy16_sized(put + j * 1024, a + j * 64, size_a);
+      copy16_sized(put + j * 1024 + 512, b + j * 64, size_b);
+    }
+    put = put == base + (kStages - 1) * kStage ? base : put + kStage;
+  }
   // Waits until the oldest stage has landed; its vectors are at the returned address.
   __device__ __forceinline__ unsigned front() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    copy_wait<kStages - 1>();
     const unsigned at = get;
     get = get == base + (kStages - 1) * kStage ? base : get + kStage;
     return at;
@@ -379,18 +421,69 @@ struct Fifo {
 };
 
 // ---------------------------------------------------------------------------------------
-// Quantised rows: q = round(v * Q / max|v|), scale = max|v| / Q.  The product v * Q of a
-// bf16 v is exact in fp32 and the division is correctly rounded, so a quotient that lies on
-// the border between two values is seen as such.
+// Quantised rows: q = round(v * Q / top), scale = top / Q, top = max|v|.  The quotient comes
+// from a product with Q / top, which is off by 2^-23 of it at most; only where that could
+// put it on the other side of a border between two values is it divided (the product v * Q
+// of a bf16 v is exact in fp32 and the division correctly rounded, so a quotient that lies
+// on a border is seen as such).  Dividing every element took 13 us for 16 tokens of 2048.
 
+struct RowQuant {
+  float top, inv;
+};
 template <int WT>
-__device__ __forceinline__ unsigned quantise(float v, float top) {
-  if (WT == kInt8) return (unsigned)(unsigned char)(signed char)__float2int_rn(v * 127.f / top);
-  return __nv_cvt_float_to_fp8(v * 448.f / top, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ RowQuant row_quant(float top) {
+  return RowQuant{top, (WT == kInt8 ? 127.f : 448.f) / top};
 }
 template <int WT>
 __device__ __forceinline__ float quant_scale(float top) {
   return top / (WT == kInt8 ? 127.f : 448.f);
+}
+
+template <int WT>
+__device__ __noinline__ unsigned quantise_exactly(float v, float top) {
+  if (top > 1e36f) {             // v * Q must not overflow
+    v *= 0x1p-20f;
+    top *= 0x1p-20f;
+  }
+  if (WT == kInt8) return (unsigned)(unsigned char)(signed char)__float2int_rn(v * 127.f / top);
+  return __nv_cvt_float_to_fp8(v * 448.f / top, __NV_SATFINITE, __NV_E4M3);
+}
+
+// Four values, packed.
+template <int WT>
+__device__ __forceinline__ unsigned quantise4(float v0, float v1, float v2, float v3,
+                                              const RowQuant& s) {
+  const float r[4] = {v0 * s.inv, v1 * s.inv, v2 * s.inv, v3 * s.inv};
+  unsigned out;
+  bool sure;
+  if (WT == kInt8) {
+    constexpr float kRound = 12582912.f;         // 1.5 * 2^23: adding it rounds to an integer
+    float m[4];
+    sure = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = __fadd_rn(r[i], kRound);
+      sure &= fabsf(r[i] - __fsub_rn(m[i], kRound)) < 0.4999f;    // false for a NaN
+    }
+    out = __byte_perm(__byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x0040),
+                      __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040), 0x5410);
+  } else {
+    constexpr float kLow = 1.f - 0x1p-20f, kHigh = 1.f + 0x1p-20f;
+    unsigned short lo[2], hi[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      lo[i] = __nv_cvt_float2_to_fp8x2(make_float2(r[2 * i] * kLow, r[2 * i + 1] * kLow),
+                                       __NV_SATFINITE, __NV_E4M3);
+      hi[i] = __nv_cvt_float2_to_fp8x2(make_float2(r[2 * i] * kHigh, r[2 * i + 1] * kHigh),
+                                       __NV_SATFINITE, __NV_E4M3);
+    }
+    sure = lo[0] == hi[0] && lo[1] == hi[1];
+    out = lo[0] | (unsigned)lo[1] << 16;
+  }
+  if (!sure)
+    out = quantise_exactly<WT>(v0, s.top) | quantise_exactly<WT>(v1, s.top) << 8 |
+          quantise_exactly<WT>(v2, s.top) << 16 | quantise_exactly<WT>(v3, s.top) << 24;
+  return out;
 }
 
 // The bits of |v| order as |v| does, a NaN above all, so that a maximum of them keeps it.
@@ -407,72 +500,100 @@ __device__ __forceinline__ int staged_at(int T, int blk, int t, int j) {
   return (blk * T + t) * 256 + ((j ^ (t & 1)) * 64);
 }
 
-// x of the CTA's tokens in shared memory (zeros past H), quantised for 8-bit weights with the
-// scales in `xs`.  Whole CTA; ends with a barrier.
-template <int WT>
-__device__ void stage_x(const ExpertsArgs& a, unsigned char* st, float* xs) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kChunk = Kind<WT>::kChunk, kVec = Kind<WT>::kVec;
-  if (WT != kBf16) {
-    __shared__ unsigned tops[kMaxTokens];
-    if (tid < kMaxTokens) tops[tid] = 0;
-    __syncthreads();
-    const int segs = (a.H + 511) / 512;           // a warp takes 512 columns of a token
-    for (int i = warp; i < segs * a.T; i += kWarps) {
-      const int t = i / segs, at = (i - t * segs) * 512 + lane * 8;
-      const __nv_bfloat16* x = a.x + t * a.ldx + at;
-      uint4 v[2] = {};
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (at + j * 256 < a.H) v[j] = *reinterpret_cast<const uint4*>(x + j * 256);
-      unsigned top = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const unsigned u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-          top = max(top, max(u[m] << 16 & 0x7fffffffu, u[m] & 0x7fff0000u));
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) atomicMax(&tops[t], top);
-    }
-    __syncthreads();
-    if (tid < a.T) xs[tid] = clamp_top(tops[tid]);
-    __syncthreads();
+// Byte `pos` of token t's row there.
+__device__ __forceinline__ int staged_byte(int T, int t, int pos) {
+  return staged_at(T, pos >> 8, t, pos >> 6 & 3) + (pos & 63);
+}
+
+// Copies of rows of `row_bytes` (x, or the quantised x) into the staged form, zeros past
+// their ends.  Whole CTA; the caller commits, waits and synchronises.
+__device__ __forceinline__ void stage_rows(const uint8_t* rows, long long stride, int row_bytes,
+                                           int T, unsigned char* st) {
+  const unsigned to = (unsigned)__cvta_generic_to_shared(st);
+  const int per = (row_bytes + 255) / 256 * 16;
+  for (int i = threadIdx.x; i < per * T; i += kThreads) {
+    const int t = i / per, pos = (i - t * per) * 16;
+    copy16(to + staged_byte(T, t, pos), rows + t * stride + pos, pos < row_bytes);
   }
-  const int pieces = (a.H + 4 * kChunk - 1) / (4 * kChunk) * 16;   // 16 bytes each, of a token
-  for (int i = tid; i < pieces * a.T; i += kThreads) {
-    const int t = i / pieces, m = i - t * pieces;
-    uint4 o = make_uint4(0, 0, 0, 0);
-    if (m * kVec < a.H) {
-      const uint4* src = reinterpret_cast<const uint4*>(a.x + t * a.ldx + m * kVec);
-      if (WT == kBf16) {
-        o = src[0];
-      } else {
-        const float top = xs[t];
-        unsigned w[4];
+}
+
+// 8-bit weights: x that up quantises itself, in registers: T * H values at most.  Beyond
+// that prep_kernel does it once for all CTAs (13 us of 105 were spent here for 16 tokens of
+// 2048, most of it waiting for x behind the first weights).
+constexpr int kSelfX = 8192;
+constexpr int kSelfXVectors = kSelfX / 8 / kThreads;
+
+struct HeldX {
+  uint4 v[kSelfXVectors];
+  __device__ __forceinline__ void load(const ExpertsArgs& a) {
+    const int per = a.H / 8;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint4 v = src[half];
-          const unsigned u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            w[2 * half + j] =
-                quantise<WT>(__uint_as_float(u[2 * j] << 16), top) |
-                quantise<WT>(__uint_as_float(u[2 * j] & 0xffff0000u), top) << 8 |
-                quantise<WT>(__uint_as_float(u[2 * j + 1] << 16), top) << 16 |
-                quantise<WT>(__uint_as_float(u[2 * j + 1] & 0xffff0000u), top) << 24;
-        }
-        o = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+    for (int j = 0; j < kSelfXVectors; ++j) {
+      const int i = threadIdx.x + j * kThreads, t = i / per;
+      v[j] = make_uint4(0, 0, 0, 0);
+      if (t < a.T) v[j] = *reinterpret_cast<const uint4*>(a.x + t * a.ldx + (i - t * per) * 8);
     }
-    *reinterpret_cast<uint4*>(st + staged_at(a.T, m >> 4, t, m >> 2 & 3) + (m & 3) * 16) = o;
+  }
+};
+
+__device__ __forceinline__ float low_bf16(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_bf16(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+__device__ __forceinline__ unsigned top_bits(const uint4& v) {
+  const unsigned u[4] = {v.x, v.y, v.z, v.w};
+  unsigned top = 0;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) top = max(top, max(u[m] << 16 & 0x7fffffffu, u[m] & 0x7fff0000u));
+  return top;
+}
+
+template <int WT>
+__device__ __forceinline__ uint2 quantise8(const uint4& v, const RowQuant& s) {
+  return make_uint2(
+      quantise4<WT>(low_bf16(v.x), high_bf16(v.x), low_bf16(v.y), high_bf16(v.y), s),
+      quantise4<WT>(low_bf16(v.z), high_bf16(v.z), low_bf16(v.w), high_bf16(v.w), s));
+}
+
+// The held x, quantised, into the staged form.  Whole CTA; ends with a barrier.
+template <int WT>
+__device__ void stage_held(const ExpertsArgs& a, const HeldX& x, unsigned char* st, float* xs) {
+  __shared__ unsigned tops[kMaxTokens];
+  __shared__ float inv[kMaxTokens];
+  const int tid = threadIdx.x, lane = tid & 31, per = a.H / 8;
+  if (tid < kMaxTokens) tops[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kSelfXVectors; ++j) {
+    const int t = (tid + j * kThreads) / per;
+    const unsigned top = top_bits(x.v[j]);
+    if (__all_sync(0xffffffffu, t == __shfl_sync(0xffffffffu, t, 0))) {
+      const unsigned m = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0 && t < a.T) atomicMax(&tops[t], m);
+    } else if (t < a.T) {
+      atomicMax(&tops[t], top);
+    }
   }
   __syncthreads();
-  if (WT != kBf16) {
-    if (tid < a.T) xs[tid] = quant_scale<WT>(xs[tid]);
-    __syncthreads();
+  if (tid < a.T) {
+    const float top = clamp_top(tops[tid]);
+    tops[tid] = __float_as_uint(top);
+    inv[tid] = row_quant<WT>(top).inv;
+    xs[tid] = quant_scale<WT>(top);
   }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kSelfXVectors; ++j) {
+    const int i = tid + j * kThreads, t = i / per;
+    if (t < a.T)
+      *reinterpret_cast<uint2*>(st + staged_byte(a.T, t, (i - t * per) * 8)) =
+          quantise8<WT>(x.v[j], RowQuant{__uint_as_float(tops[t]), inv[t]});
+  }
+  const int tail = (a.H + 255) / 256 * 256 - a.H;            // zeros, 16 bytes at a time
+  for (int i = tid; i < tail / 16 * a.T; i += kThreads) {
+    const int t = i / (tail / 16), pos = a.H + (i - t * (tail / 16)) * 16;
+    *reinterpret_cast<uint4*>(st + staged_byte(a.T, t, pos)) = make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
 }
 
 // A sum as two bf16 values (an infinite high part has no remainder).
@@ -493,14 +614,55 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
 }
 
 // ---------------------------------------------------------------------------------------
-// u[p] = c A13[adapter, expert] x[t]: one warp per row of A13.
+// prep: what up needs of x for many rows.  The first `prepared ? T : 0` CTAs quantise a token
+// each; the others, with adapters, compute u[p] = c A13[adapter, expert] x[t], a warp a row.
 
-__global__ void __launch_bounds__(kThreads) shrink_kernel(const __grid_constant__ ExpertsArgs a) {
+template <int WT, bool LORA>
+__global__ void __launch_bounds__(kThreads) prep_kernel(const __grid_constant__ ExpertsArgs a) {
   grid_dependency_wait();
   release_dependents();
-  const int p = blockIdx.x, lane = threadIdx.x & 31;
-  const int row = blockIdx.y * kWarps + (threadIdx.x >> 5);
-  const int rows = 2 * a.lora.r;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int block = blockIdx.x;
+  if (WT != kBf16 && a.prepared) {
+    if (block < a.T) {
+      __shared__ unsigned tops[kWarps];
+      const __nv_bfloat16* x = a.x + block * a.ldx;
+      uint4 held[4];                             // rows of up to 8192 are read once
+      unsigned top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = (tid + j * kThreads) * 8;
+        held[j] = make_uint4(0, 0, 0, 0);
+        if (i < a.H) held[j] = *reinterpret_cast<const uint4*>(x + i);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, top_bits(held[j]));
+      for (int i = (tid + 4 * kThreads) * 8; i < a.H; i += kThreads * 8)
+        top = max(top, top_bits(*reinterpret_cast<const uint4*>(x + i)));
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) tops[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
+      const float m = clamp_top(top);
+      const RowQuant s = row_quant<WT>(m);
+      uint8_t* to = a.xq + (size_t)block * a.H;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = (tid + j * kThreads) * 8;
+        if (i < a.H) *reinterpret_cast<uint2*>(to + i) = quantise8<WT>(held[j], s);
+      }
+      for (int i = (tid + 4 * kThreads) * 8; i < a.H; i += kThreads * 8)
+        *reinterpret_cast<uint2*>(to + i) =
+            quantise8<WT>(*reinterpret_cast<const uint4*>(x + i), s);
+      if (tid == 0) a.x_scale[block] = quant_scale<WT>(m);
+      return;
+    }
+    block -= a.T;
+  }
+  if (!LORA) return;
+  const int rows = 2 * a.lora.r, per = (rows + kWarps - 1) / kWarps;
+  const int p = block / per, row = (block - p * per) * kWarps + warp;
   if (row >= rows || slot_of(a, p) < 0) return;
   const int m = matrix_of(a, p);
   if (m < 0) return;
@@ -541,24 +703,33 @@ template <int WT, int NT, bool LORA, bool STAGED>
 __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
   using Acc = typename K::Acc;
-  constexpr int KB = 4;
+  constexpr int KB = kUpBlock;
+  using Stream = Fifo<KB, kUpStages>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  Fifo<KB> fifo(smem);
-  const Routing rt = routing_at(smem + kFifoBytes, P, NT);
-  float* xs = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT, LORA));
+  Stream fifo(smem);
+  const Routing rt = routing_at(smem + kUpFifo, P, NT);
+  float* xs = reinterpret_cast<float*>(smem + kUpFifo + routing_bytes(P, NT, LORA));
   unsigned char* st = reinterpret_cast<unsigned char*>(xs + kMaxTokens);
 
-  // With adapters shrink_kernel runs before this one; it starts this grid once its own wait
-  // is over, so the call's inputs are complete and only its result is waited for, below.
-  if (!LORA) grid_dependency_wait();
+  // Where prep_kernel runs before this one, it starts this grid once its own wait is over, so
+  // the call's inputs are complete and only its results are waited for, below.
+  const bool after_prep = LORA || (WT != kBf16 && a.prepared);
+  if (!after_prep) grid_dependency_wait();
   release_dependents();
-  build_routing<NT, LORA>(a, rt);
+  HeldX held;
+  if (WT == kBf16 && STAGED) {
+    stage_rows(reinterpret_cast<const uint8_t*>(a.x), a.ldx * 2, a.H * 2, a.T, st);
+    copy_commit();
+  }
+  if (WT != kBf16 && !a.prepared) held.load(a);
+  build_routing<NT, LORA>(a, rt, reinterpret_cast<int*>(smem));
   const int D = rt.entries[0];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const long long R = (long long)D * a.I, W = (long long)gridDim.x * kWarps;
-  const int w = blockIdx.x * kWarps + warp;
-  const int r0 = (int)(R * w / W), r1 = (int)(R * (w + 1) / W);
+  // Shares differ by a row at most, and so do the CTAs' sums of them.
+  const unsigned R = D * a.I, W = gridDim.x * kWarps, w = warp * gridDim.x + blockIdx.x;
+  const unsigned share = R / W, rest = R - share * W;
+  const int r0 = share * w + min(w, rest), r1 = r0 + share + (w < rest);
   const int row_bytes = a.H * K::kItem, lora_bytes = LORA ? a.lora.r * 2 : 0;
   const long long up_off = (long long)a.I * row_bytes;
 
@@ -578,8 +749,13 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
     if (head.row < r1) {
       const bool mine = g < head.n;
       if (!LORA || pos < row_bytes) {
-        const int left = mine ? row_bytes - pos - q * 16 : 0;
-        fifo.push(src, left, src + up_off, left);
+        if (pos + KB * 64 <= row_bytes) {
+          const int size = mine ? 16 : 0;
+          fifo.push_whole(src, size, src + up_off, size);
+        } else {
+          const int left = mine ? row_bytes - pos - q * 16 : 0;
+          fifo.push(src, left, src + up_off, left);
+        }
         src += KB * 64;
         pos += KB * 64;
       } else {
@@ -606,20 +782,30 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   };
   head.row = r1;
   if (r0 < r1) head_at(r0);
-  for (int i = 0; i < Fifo<KB>::kStages; ++i) push();
+  for (int i = 0; i < Stream::kStages; ++i) push();
 
-  if (STAGED) stage_x<WT>(a, st, xs);
-  if (LORA) grid_dependency_wait();
+  if (WT != kBf16 && !a.prepared) stage_held<WT>(a, held, st, xs);
+  if (after_prep) grid_dependency_wait();
+  if (WT != kBf16 && a.prepared) {
+    stage_rows(a.xq, a.H, a.H, a.T, st);
+    copy_commit();
+    if (tid < a.T) xs[tid] = __ldcg(a.x_scale + tid);
+    copy_wait<0>();
+    __syncthreads();
+  }
+  if (WT == kBf16 && STAGED) {       // x was copied before the stages
+    copy_wait<Stream::kStages>();
+    __syncthreads();
+  }
 
   // Column g's token of each column tile.  Past the last token: any (the column is not kept).
-  unsigned xa[NT], xb[NT];                      // staged: even and odd chunks
+  const unsigned char *xa[NT], *xb[NT];         // staged: even and odd chunks
   const __nv_bfloat16* xg[NT];                  // not staged: the row in global memory
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int t = min(nt * 8 + g, a.T - 1);
-    const unsigned at = (unsigned)__cvta_generic_to_shared(st) + q * 16;
-    xa[nt] = at + staged_at(a.T, 0, t, 0);
-    xb[nt] = at + staged_at(a.T, 0, t, 1);
+    xa[nt] = st + q * 16 + staged_at(a.T, 0, t, 0);
+    xb[nt] = st + q * 16 + staged_at(a.T, 0, t, 1);
     xg[nt] = a.x + t * a.ldx + q * 8;
   }
 
@@ -636,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       su = a.s13[(long long)slot * 2 * a.I + a.I + r];
     }
     Acc acc[NT][4] = {};
-    for (int at = 0, blk = 0; at < row_bytes; at += KB * 64, blk += a.T * 256) {
+    for (int at = 0, blk = 0; at < row_bytes; at += KB * 64) {
       const unsigned f = fifo.front();
       uint4 wa[KB], wb[KB];
 #pragma unroll
@@ -653,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
           if (NT > 1 && !(mask >> nt & 1)) continue;
           uint4 v;
           if constexpr (STAGED) {
-            v = load_shared((j & 1 ? xb[nt] : xa[nt]) + blk + (j & 2) * 64);
+            v = *reinterpret_cast<const uint4*>((j & 1 ? xb[nt] : xa[nt]) + blk + (j & 2) * 64);
           } else {
             v = make_uint4(0, 0, 0, 0);
             if (at + j * 64 + q * 16 < row_bytes)
@@ -665,6 +851,8 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
         }
       }
       push();      // into the stage just read, whose vectors the products have taken
+      if (KB == 4 || (at & 128)) blk += a.T * 256 - (KB == 2 ? 128 : 0);
+      else blk += 128;
     }
     // Adapters: one more product for each adapted column, B13's rows with u in that column
     // alone.  Gate and up have different u, so each takes its half of the 16 rows.
@@ -749,12 +937,11 @@ __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ E
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
     const float m = clamp_top(top);
+    const RowQuant rq = row_quant<WT>(m);
     if (tid == 0) a.h_scale[p] = quant_scale<WT>(m) * a.weights[p];
     for (int i = tid * 4; i < a.I; i += kThreads * 4) {
       const float4 v = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
-      *reinterpret_cast<unsigned*>(a.hq + at + i) =
-          quantise<WT>(v.x, m) | quantise<WT>(v.y, m) << 8 | quantise<WT>(v.z, m) << 16 |
-          quantise<WT>(v.w, m) << 24;
+      *reinterpret_cast<unsigned*>(a.hq + at + i) = quantise4<WT>(v.x, v.y, v.z, v.w, rq);
     }
   }
   if (!LORA) return;
@@ -795,218 +982,364 @@ __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ E
 // ---------------------------------------------------------------------------------------
 // down
 
-// Where a warp is in the stream of a CTA's rows: a tile of up to 16 rows after the other, in
-// each the CB blocks of every entry and then, as entries from D on, the RB blocks of every
-// adapted pair; the warps take these blocks in turn.
-struct DownCursor {
-  int row, n, e, c;
-  int r1, CB, D, RB, N;       // N = entries + adapted pairs
-  __device__ __forceinline__ void start(int r) {
-    row = r;
-    const int left = r1 - r, tiles = (left + 15) / 16;
-    n = tiles ? (left + tiles - 1) / tiles : 0;
-    e = 0;
-    c = threadIdx.x >> 5;
-    wrap();
+// A CTA owns a range of out's columns, taken in tiles of up to 16 (rows of W2).  Within a
+// tile a warp takes every kWarps-th unit: a slice of an entry's rows, its blocks one after
+// the other, with the accumulators kept over all units; then every kWarps-th adapted pair.
+// Entries are sliced only as far as it takes to give the warps equal shares.
+struct DownUnits {
+  int entries, log_slices, blocks, units;       // units of all entries
+  int pairs, pair_blocks;                       // adapted pairs after them
+  __device__ __forceinline__ void plan(int D, int CB, int adapted, int RB) {
+    entries = D;
+    blocks = CB;
+    log_slices = 0;
+    while ((D << log_slices) % kWarps != 0 && (D << log_slices) < 4 * kWarps &&
+           (2 << log_slices) <= CB)
+      ++log_slices;
+    units = D << log_slices;
+    pairs = adapted;
+    pair_blocks = RB;
   }
-  __device__ __forceinline__ void wrap() {
-    while (e < N && c >= (e < D ? CB : RB)) { c -= e < D ? CB : RB; ++e; }
+  __device__ __forceinline__ int all() const { return units + pairs; }
+  __device__ __forceinline__ int entry(int u) const { return u >> log_slices; }
+  // First block of unit u (of u + 1: its end).
+  __device__ __forceinline__ int first(int u) const {
+    return (u & ((1 << log_slices) - 1)) * blocks >> log_slices;
   }
-  __device__ __forceinline__ bool in_tile() const { return e < N; }
-  // On to the next tile where this one is done; false after the last.
-  __device__ __forceinline__ bool settle() {
-    while (e >= N) {
-      if (row + n >= r1) return false;
-      start(row + n);
+  __device__ __forceinline__ int end(int u) const {
+    return ((u & ((1 << log_slices) - 1)) + 1) * blocks >> log_slices;
+  }
+};
+__device__ __forceinline__ int tile_rows(int row, int r1) {
+  const int left = r1 - row, tiles = (left + 15) / 16;
+  return tiles ? (left + tiles - 1) / tiles : 0;
+}
+
+// Chunks per block: where the other operand comes from global memory, two blocks of it have
+// to fit the registers.
+template <int WT, int NT, bool HS>
+constexpr int kDownBlock = HS ? 4 : WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
+
+// h in shared memory (HS): a row of `stride` bytes (an odd number of 64: lanes of two rows
+// then read all banks) for each pair's h, two for its high and low parts, zeros past a row's
+// end; and such rows of zeros for the columns without a pair.
+__host__ __device__ inline int h_stride(int I, int wtype) {
+  return (I * (wtype == kBf16 ? 2 : 1) + 255) / 256 * 256 + 64;
+}
+__host__ __device__ inline int align16(int n) { return (n + 15) / 16 * 16; }
+// Bytes of: the pairs' scales; the scales of the CTA's `rows` of every entry; adapters' v.
+__host__ __device__ inline int pair_scale_bytes(int P, int wtype) {
+  return wtype == kBf16 ? 0 : align16(P * 4);
+}
+__host__ __device__ inline int row_scale_bytes(int P, int rows, int wtype) {
+  return wtype == kBf16 ? 0 : align16(P * rows * 4);
+}
+__host__ __device__ inline size_t h_bytes(int P, int I, int rows, int r, int wtype) {
+  return (size_t)(P + 1) * (wtype == kBf16 ? 2 : 1) * h_stride(I, wtype) +
+         pair_scale_bytes(P, wtype) + row_scale_bytes(P, rows, wtype) + (size_t)P * 2 * r * 2;
+}
+// Rows that down quantises itself: few enough that every CTA doing so costs less than a
+// launch in between.
+constexpr int kSelfWidth = 1024, kSelfValues = 16384;
+__host__ __device__ inline bool quantises_itself(int P, int I) {
+  return I <= kSelfWidth && P * I <= kSelfValues;
+}
+
+// Whole CTA; ends with a barrier, all earlier copies landed.
+template <int WT, bool LORA>
+__device__ void stage_h(const ExpertsArgs& a, const Routing& rt, unsigned char* hs, float* scale,
+                        __nv_bfloat16* v) {
+  const int P = a.T * a.k, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int stride = h_stride(a.I, WT), parts = WT == kBf16 ? 2 : 1;
+  if (LORA) {              // rows [2p] high, [2p + 1] low parts of v
+    const int per = a.lora.r / 8;
+    for (int i = tid; i < P * 2 * per; i += kThreads) {
+      const int row = i / per, at = (i - row * per) * 8, p = row >> 1;
+      if (rt.pair_slot[p] < 0 || rt.matrix[p] < 0) continue;
+      copy16((unsigned)__cvta_generic_to_shared(v + (size_t)row * a.lora.r + at),
+             reinterpret_cast<const uint8_t*>((row & 1 ? a.v_lo : a.v_hi) +
+                                              (size_t)p * a.lora.r + at), true);
     }
-    return true;
+    copy_commit();
   }
-  __device__ __forceinline__ void next() {
-    c += kWarps;
-    wrap();
+  for (int i = tid * 16; i < stride * parts; i += kThreads * 16)
+    *reinterpret_cast<uint4*>(hs + (size_t)P * parts * stride + i) = make_uint4(0, 0, 0, 0);
+  if (WT != kBf16 && quantises_itself(P, a.I)) {
+    for (int p = warp; p < P; p += kWarps) {
+      if (rt.pair_slot[p] < 0) continue;
+      float4 x[kSelfWidth / 128];
+      unsigned top = 0;
+#pragma unroll
+      for (int j = 0; j < kSelfWidth / 128; ++j) {
+        const int i = j * 128 + lane * 4;
+        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < a.I) x[j] = __ldcg(reinterpret_cast<const float4*>(a.h + (size_t)p * a.I + i));
+      }
+#pragma unroll
+      for (int j = 0; j < kSelfWidth / 128; ++j)
+        top = max(top, max(max(abs_bits(x[j].x), abs_bits(x[j].y)),
+                           max(abs_bits(x[j].z), abs_bits(x[j].w))));
+      const float m = clamp_top(__reduce_max_sync(0xffffffffu, top));
+      const RowQuant rq = row_quant<WT>(m);
+#pragma unroll
+      for (int j = 0; j < kSelfWidth / 128; ++j) {
+        const int i = j * 128 + lane * 4;
+        if (i < stride - 64)
+          *reinterpret_cast<unsigned*>(hs + (size_t)p * stride + i) =
+              i < a.I ? quantise4<WT>(x[j].x, x[j].y, x[j].z, x[j].w, rq) : 0;
+      }
+      if (lane == 0) scale[p] = quant_scale<WT>(m) * a.weights[p];
+    }
+  } else {
+    const int row_bytes = a.I * Kind<WT>::kItem, per = (stride - 64) / 16;
+    for (int i = tid; i < P * parts * per; i += kThreads) {
+      const int row = i / per, at = (i - row * per) * 16, p = row / parts;
+      if (rt.pair_slot[p] < 0) continue;
+      const uint8_t* src = WT == kBf16 ? reinterpret_cast<const uint8_t*>(row & 1 ? a.h_lo : a.h_hi)
+                                       : a.hq;
+      copy16((unsigned)__cvta_generic_to_shared(hs + (size_t)row * stride + at),
+             src + (size_t)p * row_bytes + at, at < row_bytes);
+    }
+    copy_commit();
+    if (WT != kBf16)
+      for (int p = tid; p < P; p += kThreads)
+        if (rt.pair_slot[p] >= 0) scale[p] = __ldcg(a.h_scale + p);
   }
-};
-
-// Chunks per block: the other operand of two blocks has to fit the registers.
-template <int WT, int NT>
-constexpr int kDownBlock = WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
-
-// The other operand of a block, read from L2 while the block before it is multiplied.
-template <int WT, int NT, bool LORA>
-struct DownOperand {
-  static constexpr int KB = kDownBlock<WT, NT>;
-  // of an adapter's block: chunks (their hi and lo parts take two vectors each)
-  static constexpr int LB = WT == kBf16 ? KB : KB / 2;
-  uint4 v[NT][WT == kBf16 ? 2 * KB : KB];
-  float rf[2], cf[NT][2];       // 8-bit: scales of rows g, g + 8 and of columns 2q, 2q + 1
-};
+  copy_wait<0>();
+  __syncthreads();
+}
 
 template <int NT>
 constexpr int kRed = kWarps * 16 * 8 * NT;   // the warps' partial sums
 
-template <int WT, int NT, bool LORA>
+template <int WT, int NT, bool LORA, bool HS>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
-  using Operand = DownOperand<WT, NT, LORA>;
-  constexpr int KB = Operand::KB, LB = Operand::LB;
+  using Acc = typename K::Acc;
+  constexpr int KB = kDownBlock<WT, NT, HS>, kParts = WT == kBf16 ? 2 : 1;
+  using Stream = Fifo<KB, kDownChunks / KB>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  Fifo<KB> fifo(smem);
-  const Routing rt = routing_at(smem + kFifoBytes, P, NT);
-  float* red = reinterpret_cast<float*>(smem + kFifoBytes + routing_bytes(P, NT, LORA));
+  const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
+  const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x), rows = r1 - r0;
+  Stream fifo(smem);
+  const Routing rt = routing_at(smem + kDownFifo, P, NT);
+  float* red = reinterpret_cast<float*>(smem + kDownFifo + routing_bytes(P, NT, LORA));
+  unsigned char* hs = reinterpret_cast<unsigned char*>(red + kRed<NT>);        // HS
+  const int stride = h_stride(a.I, WT);
+  unsigned char* after_h = hs + (size_t)(P + 1) * kParts * stride;
+  float* scale = reinterpret_cast<float*>(after_h);
+  float* row_scale = reinterpret_cast<float*>(after_h + pair_scale_bytes(P, WT));
+  __nv_bfloat16* vs = reinterpret_cast<__nv_bfloat16*>(after_h + pair_scale_bytes(P, WT) +
+                                                       row_scale_bytes(P, rows, WT));
 
   // Everything up to the wait reads the call's inputs only.  They are complete: this grid
   // starts once every CTA of the kernels before it has started, the first of them after its
   // own wait.
   release_dependents();
-  const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
-  const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x);
-  build_routing<NT, LORA>(a, rt);
-  const int D = rt.entries[0];
+  build_routing<NT, LORA>(a, rt, reinterpret_cast<int*>(smem));
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int row_bytes = a.I * K::kItem, lora_bytes = LORA ? a.lora.r * 2 : 0;
+  DownUnits units;
+  units.plan(rt.entries[0], (row_bytes + KB * 64 - 1) / (KB * 64), LORA ? rt.entries[2] : 0,
+             (lora_bytes + KB * 64 - 1) / (KB * 64));
+  const int U = units.all();
 
-  DownCursor head;
-  head.r1 = r1;
-  head.CB = (row_bytes + KB * 64 - 1) / (KB * 64);
-  head.D = D;
-  head.RB = LORA ? (lora_bytes + LB * 64 - 1) / (LB * 64) : 1;
-  head.N = D + (LORA ? rt.entries[2] : 0);
-  bool more = r0 < r1 && head.N > 0;
-  head.start(r0);
+  // The head of the stream: a block of unit hu of the tile at hrow.
+  int hrow = warp < U ? r0 : r1, hn = tile_rows(r0, r1), hu = warp, hb = 0, hend = 0;
+  int size_a = 0, size_b = 0, hbytes = 0;
+  const uint8_t* src = nullptr;
+  const auto head_at = [&]() {
+    size_a = g < hn ? 16 : 0;
+    size_b = g + 8 < hn ? 16 : 0;
+    if (!LORA || hu < units.units) {
+      hb = units.first(hu);
+      hend = units.end(hu);
+      hbytes = row_bytes;
+      src = a.w2 + ((long long)rt.slot[units.entry(hu)] * a.H + hrow + g) * row_bytes;
+    } else {
+      hb = 0;
+      hend = units.pair_blocks;
+      hbytes = lora_bytes;
+      src = reinterpret_cast<const uint8_t*>(a.lora.b2) +
+            ((long long)rt.matrix[rt.list[hu - units.units]] * a.H + hrow + g) * lora_bytes;
+    }
+    src += hb * (KB * 64) + q * 16;
+  };
   const auto push = [&]() {
-    if (more && (more = head.settle())) {
-      const uint8_t* src;
-      int left, stride;
-      if (!LORA || head.e < D) {
-        const int at = head.c * (KB * 64) + q * 16;
-        src = a.w2 + ((long long)rt.slot[head.e] * a.H + head.row + g) * row_bytes + at;
-        left = row_bytes - at;
-        stride = row_bytes;
+    if (hrow < r1) {
+      const uint8_t* src_b = src + 8 * hbytes;
+      if ((hb + 1) * (KB * 64) <= hbytes) {
+        fifo.push_whole(src, size_a, src_b, size_b);
       } else {
-        const int at = head.c * (LB * 64) + q * 16;
-        src = reinterpret_cast<const uint8_t*>(a.lora.b2) +
-              ((long long)rt.matrix[rt.list[head.e - D]] * a.H + head.row + g) * lora_bytes + at;
-        left = min(lora_bytes - at, LB * 64);
-        stride = lora_bytes;
+        const int left = hbytes - hb * (KB * 64) - q * 16;
+        fifo.push(src, size_a ? left : 0, src_b, size_b ? left : 0);
       }
-      fifo.push(src, g < head.n ? left : 0, src + 8LL * stride, g + 8 < head.n ? left : 0);
-      head.next();
+      src += KB * 64;
+      if (++hb == hend) {
+        hu += kWarps;
+        if (hu >= U) {
+          hu = warp;
+          hrow += hn;
+          hn = tile_rows(hrow, r1);
+        }
+        if (hrow < r1) head_at();
+      }
     }
     copy_commit();
   };
-  DownCursor at = head;
-  for (int i = 0; i < Fifo<KB>::kStages; ++i) push();
+  if (hrow < r1) head_at();
+  for (int i = 0; i < Stream::kStages; ++i) push();
+  if (HS && WT != kBf16) {
+    const int n = rt.entries[0] * rows;
+    for (int i = tid; i < n; i += kThreads) {
+      const int e = i / rows;
+      row_scale[i] = a.s2[(long long)rt.slot[e] * a.H + r0 + (i - e * rows)];
+    }
+  }
 
   grid_dependency_wait();
-  const auto fetch = [&](const DownCursor& at, Operand& o) {
-    if (LORA && at.e >= D) {
-      const int p = rt.list[at.e - D], t = p / a.k, pos = at.c * (LB * 64) + q * 16;
-      const size_t i = (size_t)p * a.lora.r + pos / 2;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < LB; ++j) {
-          const bool here = (NT == 1 || t >> 3 == nt) && g == (t & 7) && pos + j * 64 < lora_bytes;
-          o.v[nt][2 * j] = load_or_zero(a.v_hi + i + j * 32, here);
-          o.v[nt][2 * j + 1] = load_or_zero(a.v_lo + i + j * 32, here);
-        }
-      return;
-    }
-    const int pos = at.c * (KB * 64) + q * 16;
-    if (WT != kBf16) {
-      const float* s2 = a.s2 + (long long)rt.slot[at.e] * a.H + at.row;
-      o.rf[0] = g < at.n ? s2[g] : 0.f;
-      o.rf[1] = g + 8 < at.n ? s2[g + 8] : 0.f;
-    }
-    const unsigned mask = rt.mask[at.e];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      if (NT > 1 && !(mask >> nt & 1)) continue;
-      const short* col = rt.col + (size_t)at.e * 8 * NT + nt * 8;
-      const int p = col[g];
-      const int left = p >= 0 ? row_bytes - pos : 0;
-      const long long i = (long long)p * row_bytes + pos;
-#pragma unroll
-      for (int j = 0; j < KB; ++j) {
-        if constexpr (WT == kBf16) {
-          o.v[nt][2 * j] = load_or_zero(reinterpret_cast<const uint8_t*>(a.h_hi) + i + j * 64, left > j * 64);
-          o.v[nt][2 * j + 1] = load_or_zero(reinterpret_cast<const uint8_t*>(a.h_lo) + i + j * 64, left > j * 64);
-        } else {
-          o.v[nt][j] = load_or_zero(a.hq + i + j * 64, left > j * 64);
-        }
-      }
-      if (WT != kBf16) {
-        const int p0 = col[2 * q], p1 = col[2 * q + 1];
-        o.cf[nt][0] = p0 >= 0 ? __ldcg(a.h_scale + p0) : 0.f;
-        o.cf[nt][1] = p1 >= 0 ? __ldcg(a.h_scale + p1) : 0.f;
-      }
-    }
-  };
-  for (int row = r0; row < r1;) {
+  if (HS) stage_h<WT, LORA>(a, rt, hs, scale, vs);
+
+  for (int row = r0, n; row < r1; row += n) {
+    n = tile_rows(row, r1);
     float acc[NT][4] = {};
-    at.start(row);
-    const int n = at.n;
-    DownCursor ahead = at;
-    Operand ops[2];
+    for (int u = warp; u < U; u += kWarps) {
+      if (LORA && u >= units.units) {
+        // an adapted pair: B2's rows with v in its token's column
+        const int p = rt.list[u - units.units], t = p / a.k;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        for (int at = 0; at < lora_bytes; at += KB * 64) {
+          const unsigned f = fifo.front();
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-      if (ahead.in_tile()) { fetch(ahead, ops[b]); ahead.next(); }
-    while (at.in_tile()) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (!at.in_tile()) break;
-        Operand& now = ops[b];
-        const unsigned f = fifo.front();
-        if (LORA && at.e >= D) {
-#pragma unroll
-          for (int j = 0; j < LB; ++j) {
+          for (int j = 0; j < KB; ++j) {
+            const int pos = at + j * 64 + q * 16;
+            const bool in = g == (t & 7) && pos < lora_bytes;
+            uint4 hi = zero, lo = zero;
+            if (HS) {
+              if (in) {
+                const __nv_bfloat16* from = vs + (size_t)p * 2 * a.lora.r + pos / 2;
+                hi = *reinterpret_cast<const uint4*>(from);
+                lo = *reinterpret_cast<const uint4*>(from + a.lora.r);
+              }
+            } else {
+              hi = load_or_zero(a.v_hi + (size_t)p * a.lora.r + pos / 2, in);
+              lo = load_or_zero(a.v_lo + (size_t)p * a.lora.r + pos / 2, in);
+            }
             const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][2 * j]);
-              chunk_mma_bf16(acc[nt], wa, wb, now.v[nt][2 * j + 1]);
+              const bool here = NT == 1 || t >> 3 == nt;
+              chunk_mma_bf16(acc[nt], wa, wb, here ? hi : zero);
+              chunk_mma_bf16(acc[nt], wa, wb, here ? lo : zero);
             }
           }
-        } else {
-          const unsigned mask = rt.mask[at.e];
-          typename K::Acc part[NT][4] = {};
-          uint4 wa[KB], wb[KB];
+          push();
+        }
+        continue;
+      }
+      const int e = units.entry(u), end = units.end(u);
+      int b = units.first(u);
+      const unsigned mask = rt.mask[e];
+      const short* col = rt.col + (size_t)e * 8 * NT;
+      // 8-bit: scales of rows g, g + 8 and of columns 2q, 2q + 1
+      float rf[2] = {}, cf[NT][2] = {};
+      if (WT != kBf16) {
+        const float* from = HS ? row_scale + e * rows + (row - r0)
+                               : a.s2 + (long long)rt.slot[e] * a.H + row;
+        if (g < n) rf[0] = from[g];
+        if (g + 8 < n) rf[1] = from[g + 8];
+      }
+      // column g's h (its low part at `low` bytes), in shared or in global memory
+      const unsigned char* from[NT];
+      bool has[NT];
+      const long long low = HS ? stride
+                               : reinterpret_cast<const unsigned char*>(a.h_lo) -
+                                     reinterpret_cast<const unsigned char*>(a.h_hi);
 #pragma unroll
-          for (int j = 0; j < KB; ++j) {
-            wa[j] = load_shared(f + j * 1024);
-            wb[j] = load_shared(f + j * 1024 + 512);
-          }
+      for (int nt = 0; nt < NT; ++nt) {
+        const int p = col[nt * 8 + g];
+        has[nt] = p >= 0;
+        if (HS)
+          from[nt] = hs + (p >= 0 ? p : P) * kParts * stride + b * (KB * 64) + q * 16;
+        else
+          from[nt] = (WT == kBf16 ? reinterpret_cast<const unsigned char*>(a.h_hi) : a.hq) +
+                     (long long)p * row_bytes + b * (KB * 64) + q * 16;
+        if (WT != kBf16) {
+          const int p0 = col[nt * 8 + 2 * q], p1 = col[nt * 8 + 2 * q + 1];
+          if (p0 >= 0) cf[nt][0] = HS ? scale[p0] : __ldcg(a.h_scale + p0);
+          if (p1 >= 0) cf[nt][1] = HS ? scale[p1] : __ldcg(a.h_scale + p1);
+        }
+      }
+      // not HS: the operand of the next block is on its way while this one is multiplied
+      uint4 next[HS ? 1 : NT][HS ? 1 : KB][HS ? 1 : kParts];
+      const auto fetch = [&](int b) {
 #pragma unroll
-          for (int j = 0; j < KB; ++j) {
-            Wide fa, fb;
-            if (WT == kFp8) { fa = widen(wa[j]); fb = widen(wb[j]); }
+        for (int nt = 0; nt < (HS ? 0 : NT); ++nt) {
+          if (NT > 1 && !(mask >> nt & 1)) continue;
+          const int left = has[nt] && b < end ? row_bytes - b * (KB * 64) - q * 16 : 0;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (NT > 1 && !(mask >> nt & 1)) continue;
-              if constexpr (WT == kBf16) {
-                chunk_mma_bf16(acc[nt], wa[j], wb[j], now.v[nt][2 * j]);
-                chunk_mma_bf16(acc[nt], wa[j], wb[j], now.v[nt][2 * j + 1]);
-              }
-              if constexpr (WT == kInt8) chunk_mma_s8(part[nt], wa[j], wb[j], now.v[nt][j]);
-              if constexpr (WT == kFp8) chunk_mma_fp8(part[nt], fa, fb, now.v[nt][j]);
-            }
-          }
-          if (WT != kBf16) {
+          for (int j = 0; j < KB; ++j)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (NT > 1 && !(mask >> nt & 1)) continue;
-              acc[nt][0] += (float)part[nt][0] * (now.rf[0] * now.cf[nt][0]);
-              acc[nt][1] += (float)part[nt][1] * (now.rf[0] * now.cf[nt][1]);
-              acc[nt][2] += (float)part[nt][2] * (now.rf[1] * now.cf[nt][0]);
-              acc[nt][3] += (float)part[nt][3] * (now.rf[1] * now.cf[nt][1]);
+            for (int part = 0; part < kParts; ++part)
+              next[nt][j][part] = load_or_zero(from[nt] + part * low + j * 64, left > j * 64);
+          from[nt] += KB * 64;
+        }
+      };
+      if (!HS) fetch(b);
+      Acc sum[NT][4] = {};
+      for (; b < end; ++b) {
+        uint4 now[HS ? 1 : NT][HS ? 1 : KB][HS ? 1 : kParts];
+        if (!HS) {
+#pragma unroll
+          for (int nt = 0; nt < (HS ? 0 : NT); ++nt)
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) now[nt][j][part] = next[nt][j][part];
+          fetch(b + 1);
+        }
+        const unsigned f = fifo.front();
+        uint4 wa[KB], wb[KB];
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          wa[j] = load_shared(f + j * 1024);
+          wb[j] = load_shared(f + j * 1024 + 512);
+        }
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          Wide fa, fb;
+          if (WT == kFp8) { fa = widen(wa[j]); fb = widen(wb[j]); }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (NT > 1 && !(mask >> nt & 1)) continue;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              uint4 v;
+              if constexpr (HS) v = *reinterpret_cast<const uint4*>(from[nt] + part * stride + j * 64);
+              else v = now[nt][j][part];
+              if constexpr (WT == kBf16) chunk_mma_bf16(acc[nt], wa[j], wb[j], v);
+              if constexpr (WT == kInt8) chunk_mma_s8(sum[nt], wa[j], wb[j], v);
+              if constexpr (WT == kFp8) chunk_mma_fp8(sum[nt], fa, fb, v);
             }
           }
         }
+        if (HS)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if (has[nt]) from[nt] += KB * 64;
         push();
-        at.next();
-        if (ahead.in_tile()) { fetch(ahead, now); ahead.next(); }
+      }
+      if (WT != kBf16) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (NT > 1 && !(mask >> nt & 1)) continue;
+          acc[nt][0] += (float)sum[nt][0] * (rf[0] * cf[nt][0]);
+          acc[nt][1] += (float)sum[nt][1] * (rf[0] * cf[nt][1]);
+          acc[nt][2] += (float)sum[nt][2] * (rf[1] * cf[nt][0]);
+          acc[nt][3] += (float)sum[nt][3] * (rf[1] * cf[nt][1]);
+        }
       }
     }
     float* mine = red + warp * 16 * 8 * NT;
@@ -1028,7 +1361,6 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
       a.out[t * a.ldo + row + i] = __float2bfloat16(s);
     }
     __syncthreads();
-    row += n;
   }
 }
 
@@ -1206,18 +1538,18 @@ size_t staged_bytes(int T, int H, int wtype) {
 
 int column_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
 
-// Shared memory of up_kernel without the copy of x, and of down_kernel.
+// Shared memory of up_kernel without the copy of x, and of down_kernel without h.
 size_t up_bytes(int P, int NT, bool lora) {
-  return kFifoBytes + routing_bytes(P, NT, lora) + kMaxTokens * 4;
+  return kUpFifo + routing_bytes(P, NT, lora) + kMaxTokens * 4;
 }
 size_t down_bytes(int P, int NT, bool lora) {
-  return kFifoBytes + routing_bytes(P, NT, lora) + (size_t)kWarps * 16 * 8 * NT * 4;
+  return kDownFifo + routing_bytes(P, NT, lora) + (size_t)kWarps * 16 * 8 * NT * 4;
 }
 
 // Does the copy of x fit beside it?  bf16 rows are read from L1 / L2 where it does not.
 bool fits_staged(int T, int k, int H, int wtype) {
   const int NT = column_tiles(T);
-  return up_bytes(T * k, NT, true) + staged_bytes(T, H, wtype) + kMaxTokens * 4 <= kSmem;
+  return up_bytes(T * k, NT, true) + staged_bytes(T, H, wtype) + 2 * kMaxTokens * 4 <= kSmem;
 }
 
 // Tokens of one launch: as many as fit the column tiles, the pair tables and (8-bit
@@ -1232,8 +1564,10 @@ int tokens_per_launch(int T, int k, int H, int wtype) {
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-// The workspace's parts for `pairs` pairs; returns its size.
-size_t carve(ExpertsArgs* a, unsigned char* base, size_t pairs, int I, int wtype, int r) {
+// The workspace's parts for `tokens` tokens of k experts; returns its size.
+size_t carve(ExpertsArgs* a, unsigned char* base, int tokens, int k, int H, int I, int wtype,
+             int r) {
+  const size_t pairs = (size_t)tokens * k;
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     unsigned char* p = base ? base + at : nullptr;
@@ -1247,6 +1581,8 @@ size_t carve(ExpertsArgs* a, unsigned char* base, size_t pairs, int I, int wtype
     a->h = reinterpret_cast<float*>(take(pairs * I * 4));
     a->hq = take(pairs * I);
     a->h_scale = reinterpret_cast<float*>(take(pairs * 4));
+    a->xq = take((size_t)tokens * H);
+    a->x_scale = reinterpret_cast<float*>(take((size_t)tokens * 4));
   }
   if (r) {
     a->u_hi = reinterpret_cast<__nv_bfloat16*>(take(pairs * 2 * r * 2));
@@ -1259,7 +1595,7 @@ size_t carve(ExpertsArgs* a, unsigned char* base, size_t pairs, int I, int wtype
 
 template <int WT, int NT, bool LORA>
 int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
-  static std::atomic<bool> done_up[2][kMaxDevices], done_down[kMaxDevices];
+  static std::atomic<bool> done_up[2][kMaxDevices], done_down[2][kMaxDevices];
   int dev = 0, sms = 0;
   int rc = device_sms(&dev, &sms);
   if (rc != 0) return rc;
@@ -1267,23 +1603,28 @@ int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
   const bool staged = WT != kBf16 || fits_staged(a.T, a.k, a.H, WT);
   const auto up = staged ? up_kernel<WT, NT, LORA, true> : up_kernel<WT, NT, LORA, WT != kBf16>;
   cudaError_t err = allow_smem(up, done_up[staged], dev);
-  if (err == cudaSuccess) err = allow_smem(down_kernel<WT, NT, LORA>, done_down, dev);
-  if (err != cudaSuccess) return (int)err;
   const int P = a.T * a.k;
-  if (LORA) {
-    rc = launch(shrink_kernel, dim3(P, (2 * a.lora.r + kWarps - 1) / kWarps), kThreads, 0,
-                stream, a);
+  size_t down_smem = down_bytes(P, NT, LORA);
+  const size_t in_smem = h_bytes(P, a.I, (a.H + sms - 1) / sms, a.lora.r, WT);
+  const bool hs = down_smem + in_smem <= kSmem;
+  if (hs) down_smem += in_smem;
+  const auto down = hs ? down_kernel<WT, NT, LORA, true> : down_kernel<WT, NT, LORA, false>;
+  if (err == cudaSuccess) err = allow_smem(down, done_down[hs], dev);
+  if (err != cudaSuccess) return (int)err;
+  if (LORA || a.prepared) {
+    const int grid = (a.prepared ? a.T : 0) +
+                     (LORA ? P * ((2 * a.lora.r + kWarps - 1) / kWarps) : 0);
+    rc = launch(prep_kernel<WT, LORA>, dim3(grid), kThreads, 0, stream, a);
     if (rc != 0) return rc;
   }
   rc = launch(up, dim3(sms), kThreads,
               up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a);
   if (rc != 0) return rc;
-  if (WT != kBf16 || LORA) {
+  if (LORA || (WT != kBf16 && !(hs && quantises_itself(P, a.I)))) {
     rc = launch(mid_kernel<WT, LORA>, dim3(P), kThreads, 0, stream, a);
     if (rc != 0) return rc;
   }
-  return launch(down_kernel<WT, NT, LORA>, dim3(sms), kThreads, down_bytes(P, NT, LORA), stream,
-                a);
+  return launch(down, dim3(sms), kThreads, down_smem, stream, a);
 }
 
 template <int WT, bool LORA>
@@ -1325,9 +1666,9 @@ int experts_checked(ExpertsArgs a, int wtype, void* workspace, long workspace_by
       misaligned(a.ids, 4) || misaligned(a.weights, 4) || misaligned(a.map, 4))
     return -1;
   const int per = tokens_per_launch(T, a.k, a.H, wtype);
-  const size_t need = carve(&a, nullptr, (size_t)per * a.k, a.I, wtype, r);
+  const size_t need = carve(&a, nullptr, per, a.k, a.H, a.I, wtype, r);
   if (!workspace || misaligned(workspace, 256) || workspace_bytes < (long)need) return -1;
-  carve(&a, static_cast<unsigned char*>(workspace), (size_t)per * a.k, a.I, wtype, r);
+  carve(&a, static_cast<unsigned char*>(workspace), per, a.k, a.H, a.I, wtype, r);
   const ExpertsArgs all = a;
   for (int t = 0; t < T; t += per) {
     a.T = T - t < per ? T - t : per;
@@ -1336,6 +1677,7 @@ int experts_checked(ExpertsArgs a, int wtype, void* workspace, long workspace_by
     a.ids = all.ids + (long long)t * all.k;
     a.weights = all.weights + (long long)t * all.k;
     if (r) a.lora.index = all.lora.index + t;
+    a.prepared = wtype != kBf16 && (long long)a.T * a.H > kSelfX;
     const int rc = wtype == kBf16   ? run_type<kBf16>(a, stream)
                    : wtype == kInt8 ? run_type<kInt8>(a, stream)
                                     : run_type<kFp8>(a, stream);
@@ -1378,8 +1720,7 @@ int expert_cache_experts_workspace(int T, int k, int H, int I, int wtype, int r,
   if (r < 0 || r > EXPERT_CACHE_LORA_MAX_RANK || r % 8) return -1;
   ExpertsArgs a{};
   *bytes = T == 0 ? 0
-                  : (long)carve(&a, nullptr, (size_t)tokens_per_launch(T, k, H, wtype) * k, I,
-                                wtype, r);
+                  : (long)carve(&a, nullptr, tokens_per_launch(T, k, H, wtype), k, H, I, wtype, r);
   return 0;
 }
 
