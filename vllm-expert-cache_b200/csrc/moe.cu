@@ -40,7 +40,13 @@
 namespace {
 
 constexpr int kMaxDevices = 64;
-constexpr int kWarps = 8;
+#ifndef KW
+#define KW 8
+#endif
+#ifndef HSKB
+#define HSKB 4
+#endif
+constexpr int kWarps = KW;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxPairs = EXPERT_CACHE_MAX_SLOTS;   // (token, expert) pairs of one launch
 constexpr int kMaxTokens = 32;                      // tokens of one launch (4 column tiles)
@@ -335,10 +341,10 @@ __device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, cons
 #define UPKB 4
 #endif
 #ifndef UPST
-#define UPST 3
+#define UPST 4
 #endif
 #ifndef DNST
-#define DNST 12
+#define DNST 16
 #endif
 constexpr int kUpBlock = UPKB, kUpStages = UPST;
 constexpr int kUpFifo = kUpStages * kUpBlock * kThreads * 32;
@@ -683,19 +689,29 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------------------
 // up
 
-// A warp's share of the flat range of all entries' row pairs, in tiles of up to 8 rows of one
-// entry.  No warp waits for another: the tile's rows stay in one warp over their whole
-// length, so that h comes straight from the accumulators.  (Splitting a tile's columns over
-// the CTA's warps, with a barrier and a sum at every tile's end, was 1.4 times slower for
-// one token in int8.)
+// Every entry's row pairs are cut into the same number of tiles of up to 8, and the warps take
+// the tiles in turn.  The number is the largest that needs no more turns than tiles of 8 do,
+// so that all warps have as many and, within a row, equally large ones; a tile is a row pair
+// of 8 at most and never crosses into another entry (a warp whose share did had two tiles to
+// stream where the others had one, and held up the layer by 5 us of 25).  No warp waits for
+// another: the rows stay in one warp over their whole length, so that h comes straight from
+// the accumulators.
+struct UpTiles {
+  int I, per_entry, all;
+  __device__ __forceinline__ UpTiles(int D, int I_, int W) : I(I_) {
+    const int least = (I + 7) / 8;
+    const int turns = (D * least + W - 1) / W;
+    per_entry = D ? min(I, turns * W / D) : 0;
+    all = D * per_entry;
+  }
+};
 struct UpTile {
-  int row, e, i0, n;
-  __device__ __forceinline__ void at(int r, int r1, int I) {
-    row = r;
-    e = r / I;
-    i0 = r - e * I;
-    const int left = min(r1 - r, I - i0), tiles = (left + 7) / 8;
-    n = (left + tiles - 1) / tiles;
+  int e, i0, n;
+  __device__ __forceinline__ void at(const UpTiles& t, int i) {
+    e = i / t.per_entry;
+    const int j = i - e * t.per_entry;
+    i0 = (int)((long long)j * t.I / t.per_entry);
+    n = (int)((long long)(j + 1) * t.I / t.per_entry) - i0;
   }
 };
 
@@ -726,27 +742,26 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   build_routing<NT, LORA>(a, rt, reinterpret_cast<int*>(smem));
   const int D = rt.entries[0];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  // Shares differ by a row at most, and so do the CTAs' sums of them.
-  const unsigned R = D * a.I, W = gridDim.x * kWarps, w = warp * gridDim.x + blockIdx.x;
-  const unsigned share = R / W, rest = R - share * W;
-  const int r0 = share * w + min(w, rest), r1 = r0 + share + (w < rest);
+  const int W = gridDim.x * kWarps, w = warp * gridDim.x + blockIdx.x;
+  const UpTiles tiles(D, a.I, W);
   const int row_bytes = a.H * K::kItem, lora_bytes = LORA ? a.lora.r * 2 : 0;
   const long long up_off = (long long)a.I * row_bytes;
 
   // The blocks of the warp's tiles in order, those of each tile's adapted columns after them;
   // `src` and the counters follow the head of the stream.
   UpTile head;
+  int hi = w;                   // its tile
   const uint8_t* src = nullptr;
   int pos = 0;                  // bytes of the row (of B13's, past the row's end) gone by
   unsigned adapted = 0;
-  const auto head_at = [&](int row) {
-    head.at(row, r1, a.I);
+  const auto head_at = [&]() {
+    head.at(tiles, hi);
     src = a.w13 + ((long long)rt.slot[head.e] * 2 * a.I + head.i0 + g) * row_bytes + q * 16;
     pos = 0;
     if (LORA) adapted = rt.adapted[head.e];
   };
   const auto push = [&]() {
-    if (head.row < r1) {
+    if (hi < tiles.all) {
       const bool mine = g < head.n;
       if (!LORA || pos < row_bytes) {
         if (pos + KB * 64 <= row_bytes) {
@@ -773,15 +788,13 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
         }
       }
       if (pos >= row_bytes && (!LORA || adapted == 0)) {
-        const int next = head.row + head.n;
-        if (next < r1) head_at(next);
-        else head.row = r1;
+        hi += W;
+        if (hi < tiles.all) head_at();
       }
     }
     copy_commit();
   };
-  head.row = r1;
-  if (r0 < r1) head_at(r0);
+  if (hi < tiles.all) head_at();
   for (int i = 0; i < Stream::kStages; ++i) push();
 
   if (WT != kBf16 && !a.prepared) stage_held<WT>(a, held, st, xs);
@@ -810,8 +823,8 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   }
 
   UpTile tile;
-  for (int row = r0; row < r1; row += tile.n) {
-    tile.at(row, r1, a.I);
+  for (int i = w; i < tiles.all; i += W) {
+    tile.at(tiles, i);
     const int slot = rt.slot[tile.e], r = tile.i0 + g;
     const unsigned mask = rt.mask[tile.e];
     const bool mine = g < tile.n;
@@ -868,10 +881,10 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
           for (int j = 0; j < KB; ++j) {
             if (at + j * 64 >= lora_bytes) break;
             const bool has = g == (t & 7) && at + j * 64 + q * 16 < lora_bytes;
-            const size_t i = up + at / 2 + j * 32;
-            const uint4 v[4] = {load_or_zero(a.u_hi + i, has), load_or_zero(a.u_lo + i, has),
-                                load_or_zero(a.u_hi + i + a.lora.r, has),
-                                load_or_zero(a.u_lo + i + a.lora.r, has)};
+            const size_t m = up + at / 2 + j * 32;
+            const uint4 v[4] = {load_or_zero(a.u_hi + m, has), load_or_zero(a.u_lo + m, has),
+                                load_or_zero(a.u_hi + m + a.lora.r, has),
+                                load_or_zero(a.u_lo + m + a.lora.r, has)};
             const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -1018,7 +1031,7 @@ __device__ __forceinline__ int tile_rows(int row, int r1) {
 // Chunks per block: where the other operand comes from global memory, two blocks of it have
 // to fit the registers.
 template <int WT, int NT, bool HS>
-constexpr int kDownBlock = HS ? 4 : WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
+constexpr int kDownBlock = HS ? HSKB : WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
 
 // h in shared memory (HS): a row of `stride` bytes (an odd number of 64: lanes of two rows
 // then read all banks) for each pair's h, two for its high and low parts, zeros past a row's
