@@ -40,13 +40,7 @@
 namespace {
 
 constexpr int kMaxDevices = 64;
-#ifndef KW
-#define KW 8
-#endif
-#ifndef HSKB
-#define HSKB 4
-#endif
-constexpr int kWarps = KW;
+constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxPairs = EXPERT_CACHE_MAX_SLOTS;   // (token, expert) pairs of one launch
 constexpr int kMaxTokens = 32;                      // tokens of one launch (4 column tiles)
@@ -79,6 +73,7 @@ struct ExpertsArgs {
   __nv_bfloat16* out;
   long long ldx, ldo;
   int T, k, H, I, S, n_map;
+  float per_k;                     // 1 / k
   // workspace
   __nv_bfloat16 *h_hi, *h_lo;      // bf16 weights: weights[t,j] * h in two parts [P][I]
   float* h;                        // 8-bit weights: h [P][I]
@@ -87,6 +82,7 @@ struct ExpertsArgs {
   uint8_t* xq;                     // 8-bit weights: quantised x [T][H] where prep_kernel runs
   float* x_scale;                  // and its scales [T]
   int prepared;                    // prep_kernel quantises x
+  int self_h;                      // down_kernel quantises h
   __nv_bfloat16 *u_hi, *u_lo;      // adapters: c A13 x in two parts [P][2r]
   __nv_bfloat16 *v_hi, *v_lo;      // adapters: c weights[t,j] A2 h in two parts [P][r]
   Adapters lora;
@@ -132,9 +128,9 @@ __device__ __forceinline__ Routing routing_at(unsigned char* base, int P, int NT
   return r;
 }
 
-// A map of up to this many entries is copied to shared memory while the ids arrive, so that
-// the two reads do not wait for each other (each may be a miss to DRAM, 0.9 us).
-constexpr int kMapCopy = 1024;
+__device__ __forceinline__ int token_of(const ExpertsArgs& a, int p) {
+  return (int)((p + 0.5f) * a.per_k);          // p / k: exact for p < 2^16, k <= 32
+}
 
 __device__ __forceinline__ int slot_of(const ExpertsArgs& a, int p) {
   int s = a.ids[p];
@@ -144,47 +140,106 @@ __device__ __forceinline__ int slot_of(const ExpertsArgs& a, int p) {
 
 // The index of a pair's adapter among the [L][E] matrices, or -1.
 __device__ __forceinline__ int matrix_of(const ExpertsArgs& a, int p) {
-  const int l = a.lora.index[p / a.k], e = a.ids[p];
+  const int l = a.lora.index[token_of(a, p)], e = a.ids[p];
   return (l < 0 || l >= a.lora.L || e < 0 || e >= a.lora.E) ? -1 : l * a.lora.E + e;
 }
 
-// Whole CTA; ends with a barrier.  Entries are in ascending slot order (repetitions after
-// them in pair order), so sums over entries have one order.
+// The first reads of a kernel, started before anything else is done.  A map of up to
+// kMapCopy entries is copied to shared memory while the ids arrive, so that the two reads do
+// not wait for each other (each may be a miss to DRAM, 0.9 us).
+constexpr int kMapCopy = 1024;
+struct FirstReads {
+  int id, map[kMapCopy / kThreads];
+  bool copied;
+  __device__ __forceinline__ explicit FirstReads(const ExpertsArgs& a) {
+    const int tid = threadIdx.x;
+    id = tid < a.T * a.k ? a.ids[tid] : -1;
+    copied = a.map && a.n_map <= kMapCopy;
+#pragma unroll
+    for (int j = 0; j < kMapCopy / kThreads; ++j) {
+      const int i = tid + j * kThreads;
+      map[j] = copied && tid < kThreads && i < a.n_map ? a.map[i] : -1;
+    }
+  }
+};
+
+// Whole CTA (kThreads threads or more); ends with a barrier.  Entries are in ascending slot
+// order (repetitions after them in pair order), so sums over entries have one order.
 // `scratch`: kMapCopy ints that nothing else uses yet.
 template <int NT, bool LORA>
-__device__ void build_routing(const ExpertsArgs& a, const Routing& r, int* scratch) {
+__device__ void build_routing(const ExpertsArgs& a, const Routing& r, const FirstReads& first,
+                              int* scratch) {
   const int P = a.T * a.k, tid = threadIdx.x, lane = tid & 31;
   constexpr int kWords = kMaxPairs / 32;
   static_assert(kWords == 32, "a lane holds a word of the slots' bits");
   if (tid < kWords) r.bits[tid] = 0;
   if (tid == 0) r.entries[1] = r.entries[2] = 0;
-  for (int i = tid; i < P * 8 * NT / 2; i += kThreads)
+  for (int i = tid; i < P * 8 * NT / 2; i += blockDim.x)
     reinterpret_cast<int*>(r.col)[i] = -1;
-  const bool copied = a.map && a.n_map <= kMapCopy;
-  if (copied) {
+  for (int p = tid; p < P; p += blockDim.x) r.mask[p] = 0;
+  const bool copied = first.copied;
+  if (copied && tid < kThreads) {
 #pragma unroll
-    for (int j = 0; j < kMapCopy; j += kThreads)
-      if (tid + j < a.n_map) scratch[tid + j] = a.map[tid + j];
+    for (int j = 0; j < kMapCopy / kThreads; ++j) scratch[tid + j * kThreads] = first.map[j];
   }
-  int id = tid < P ? a.ids[tid] : -1;           // (in flight together with the map)
-  if (copied) __syncthreads();
-  for (int p = tid; p < P; p += kThreads) {
-    if (p != tid) id = a.ids[p];
+  __syncthreads();
+  const auto slot = [&](int id) {
     int s = id;
     if (a.map) s = (id >= 0 && id < a.n_map) ? (copied ? scratch : a.map)[id] : -1;
-    r.pair_slot[p] = (short)(s >= 0 && s < a.S ? s : -1);
-    r.mask[p] = 0;
+    return s >= 0 && s < a.S ? s : -1;
+  };
+
+  if (P <= 32) {               // one warp, no barriers in between
+    if (tid < 32) {
+      const unsigned below = (1u << lane) - 1u;
+      const int p = lane, s = p < P ? slot(first.id) : -1, t = token_of(a, p);
+      const int m = LORA && s >= 0 ? matrix_of(a, p) : -1;
+      // pairs of the same slot; one of the same token before this pair makes it a repetition
+      const unsigned same = __match_any_sync(0xffffffffu, s);
+      const unsigned mine = below & ~((1u << (t * a.k)) - 1u);     // the token's pairs before
+      const bool again = s >= 0 && (same & mine) != 0;
+      const unsigned lead = __ballot_sync(0xffffffffu, s >= 0 && (same & below) == 0);
+      const unsigned rest = __ballot_sync(0xffffffffu, again);
+      int e = 0;                                   // leading pairs with a smaller slot
+      for (unsigned b = lead; b; b &= b - 1) e += __shfl_sync(0xffffffffu, s, __ffs(b) - 1) < s;
+      if (again) e = __popc(lead) + __popc(rest & below);
+      if (p < P) r.pair_slot[p] = (short)s;
+      if (LORA && p < P) {
+        r.matrix[p] = m;
+        r.adapted[p] = 0;
+      }
+      __syncwarp();
+      if (s >= 0) {
+        r.slot[e] = (short)s;
+        r.col[e * 8 * NT + t] = (short)p;
+        if (NT == 1) r.mask[e] = 1;
+        else atomicOr(reinterpret_cast<unsigned*>(r.mask) + (e >> 2), 1u << (8 * (e & 3) + (t >> 3)));
+        if (LORA && m >= 0) atomicOr(&r.adapted[e], 1u << t);
+      }
+      if (LORA) {
+        const unsigned has = __ballot_sync(0xffffffffu, m >= 0);
+        if (m >= 0) r.list[__popc(has & below)] = (short)p;
+        if (lane == 0) r.entries[2] = __popc(has);
+      }
+      if (lane == 0) r.entries[0] = __popc(lead) + __popc(rest);
+    }
+    __syncthreads();
+    return;
+  }
+
+  for (int p = tid; p < P; p += blockDim.x) {
+    r.pair_slot[p] = (short)slot(p == tid ? first.id : a.ids[p]);
     if (LORA) {
       r.matrix[p] = matrix_of(a, p);
       r.adapted[p] = 0;
     }
   }
   __syncthreads();
-  for (int p = tid; p < P; p += kThreads) {
+  for (int p = tid; p < P; p += blockDim.x) {
     const int s = r.pair_slot[p];
     if (s < 0) continue;
     bool again = false;
-    for (int q = p - p % a.k; q < p; ++q) again |= r.pair_slot[q] == s;
+    for (int q = token_of(a, p) * a.k; q < p; ++q) again |= r.pair_slot[q] == s;
     if (again) r.entries[1] = 1;
     atomicOr(&r.bits[s >> 5], 1u << (s & 31));
   }
@@ -199,23 +254,24 @@ __device__ void build_routing(const ExpertsArgs& a, const Routing& r, int* scrat
   }
   if (tid == 31) r.entries[0] = before;
   before -= __popc(bits);
-  for (int p0 = tid - lane; p0 < P; p0 += kThreads) {
+  for (int p0 = tid - lane; p0 < P; p0 += blockDim.x) {
     const int p = p0 + lane, s = p < P ? r.pair_slot[p] : -1;
     const int word = s >= 0 ? s >> 5 : 0;
     const int base = __shfl_sync(0xffffffffu, before, word);
     const unsigned b = __shfl_sync(0xffffffffu, bits, word);
-    bool first = s >= 0;
+    const int t = token_of(a, p);
+    bool leads = s >= 0;
     if (repeats && s >= 0)
-      for (int q = p - p % a.k; q < p; ++q) first &= r.pair_slot[q] != s;
-    if (!first) continue;
-    const int e = base + __popc(b & ((1u << (s & 31)) - 1u)), t = p / a.k;
+      for (int q = t * a.k; q < p; ++q) leads &= r.pair_slot[q] != s;
+    if (!leads) continue;
+    const int e = base + __popc(b & ((1u << (s & 31)) - 1u));
     r.slot[e] = (short)s;
     r.col[(size_t)e * 8 * NT + t] = (short)p;
     if (NT == 1) r.mask[e] = 1;
     else atomicOr(reinterpret_cast<unsigned*>(r.mask) + (e >> 2), 1u << (8 * (e & 3) + (t >> 3)));
     if (LORA && r.matrix[p] >= 0) atomicOr(&r.adapted[e], 1u << t);
   }
-  if (LORA && tid >= kThreads - 32) {      // the adapted pairs in ascending order
+  if (LORA && tid >= kThreads - 32 && tid < kThreads) {   // the adapted pairs in ascending order
     int n = 0;
     for (int at = 0; at < P; at += 32) {
       const int p = at + lane;
@@ -231,10 +287,10 @@ __device__ void build_routing(const ExpertsArgs& a, const Routing& r, int* scrat
   if (tid == 0) {
     int n = r.entries[0];
     for (int p = 0; p < P; ++p) {
-      const int s = r.pair_slot[p], t = p / a.k;
-      bool first = true;
-      for (int q = p - p % a.k; q < p; ++q) first &= r.pair_slot[q] != s;
-      if (s < 0 || first) continue;
+      const int s = r.pair_slot[p], t = token_of(a, p);
+      bool leads = true;
+      for (int q = t * a.k; q < p; ++q) leads &= r.pair_slot[q] != s;
+      if (s < 0 || leads) continue;
       r.slot[n] = (short)s;
       r.col[(size_t)n * 8 * NT + t] = (short)p;
       r.mask[n] = (unsigned char)(1u << (t >> 3));
@@ -337,19 +393,11 @@ __device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, cons
 // issuing them, at 0.37 of the memory's rate.)  The FIFOs leave room for a CTA of up and one
 // of down on an SM, so that down has its tables and its first stages before up is done.
 
-#ifndef UPKB
-#define UPKB 4
-#endif
-#ifndef UPST
-#define UPST 4
-#endif
-#ifndef DNST
-#define DNST 16
-#endif
-constexpr int kUpBlock = UPKB, kUpStages = UPST;
+constexpr int kUpBlock = 4, kUpStages = 3;
 constexpr int kUpFifo = kUpStages * kUpBlock * kThreads * 32;
-constexpr int kDownChunks = DNST;              // chunks of a thread's FIFO in down
-constexpr int kDownFifo = kDownChunks * kThreads * 32;
+// Chunks of a thread's FIFO in down: without h in shared memory, with it.
+constexpr int kDownChunks[2] = {16, 12};
+constexpr int down_fifo(bool hs) { return kDownChunks[hs] * kThreads * 32; }
 
 // size 0: the vector is zero-filled and nothing is read.
 __device__ __forceinline__ void copy16_sized(unsigned dst, const uint8_t* src, int size) {
@@ -673,7 +721,8 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const __grid_constant__ 
   const int m = matrix_of(a, p);
   if (m < 0) return;
   const __nv_bfloat16* w = a.lora.a13 + ((long long)m * rows + row) * a.H;
-  const __nv_bfloat16* x = a.x + (p / a.k) * a.ldx;
+  const __nv_bfloat16* x = a.x + token_of(a, p) * a.ldx;
+  const float factor = a.lora.scaling[m / a.lora.E];
   float s = 0.f;
 #pragma unroll 8
   for (int i = lane * 8; i < a.H; i += 256)
@@ -682,7 +731,7 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const __grid_constant__ 
   for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
   if (lane == 0) {
     const size_t at = (size_t)p * rows + row;
-    split(s * a.lora.scaling[m / a.lora.E], a.u_hi + at, a.u_lo + at);
+    split(s * factor, a.u_hi + at, a.u_lo + at);
   }
 }
 
@@ -733,13 +782,14 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   const bool after_prep = LORA || (WT != kBf16 && a.prepared);
   if (!after_prep) grid_dependency_wait();
   release_dependents();
+  const FirstReads first(a);
   HeldX held;
   if (WT == kBf16 && STAGED) {
     stage_rows(reinterpret_cast<const uint8_t*>(a.x), a.ldx * 2, a.H * 2, a.T, st);
     copy_commit();
   }
   if (WT != kBf16 && !a.prepared) held.load(a);
-  build_routing<NT, LORA>(a, rt, reinterpret_cast<int*>(smem));
+  build_routing<NT, LORA>(a, rt, first, reinterpret_cast<int*>(smem));
   const int D = rt.entries[0];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int W = gridDim.x * kWarps, w = warp * gridDim.x + blockIdx.x;
@@ -928,67 +978,107 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------------------------------
-// mid: one CTA per pair
+// mid: what down needs of h and cannot make itself.  With 8-bit weights the first P CTAs
+// quantise a pair's h each (unless down does: `self_h`); the others, with
+// adapters, compute v[p] = c weights[t,j] A2[adapter, expert] h, a warp a row.  All that does not
+// hang on h is read before the wait, A2's rows too.
 
 template <int WT, bool LORA>
 __global__ void __launch_bounds__(kThreads) mid_kernel(const __grid_constant__ ExpertsArgs a) {
   release_dependents();       // down may start streaming: it waits for this kernel's end
-  grid_dependency_wait();
-  const int p = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (slot_of(a, p) < 0) return;
-  const size_t at = (size_t)p * a.I;
-  if (WT != kBf16) {
-    __shared__ unsigned tops[kWarps];
-    unsigned top = 0;
-    for (int i = tid * 4; i < a.I; i += kThreads * 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
-      top = max(max(top, max(abs_bits(v.x), abs_bits(v.y))), max(abs_bits(v.z), abs_bits(v.w)));
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) tops[warp] = top;
-    __syncthreads();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int P = a.T * a.k;
+  int block = blockIdx.x;
+  if (WT != kBf16 && !a.self_h) {
+    if (block < P) {
+      const int p = block;
+      const bool has = slot_of(a, p) >= 0;
+      const float weight = a.weights[p];
+      grid_dependency_wait();
+      if (!has) return;
+      const size_t at = (size_t)p * a.I;
+      __shared__ unsigned tops[kWarps];
+      unsigned top = 0;
+      float4 held[4];                            // rows of up to 4096 are read once
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
-    const float m = clamp_top(top);
-    const RowQuant rq = row_quant<WT>(m);
-    if (tid == 0) a.h_scale[p] = quant_scale<WT>(m) * a.weights[p];
-    for (int i = tid * 4; i < a.I; i += kThreads * 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
-      *reinterpret_cast<unsigned*>(a.hq + at + i) = quantise4<WT>(v.x, v.y, v.z, v.w, rq);
+      for (int j = 0; j < 4; ++j) {
+        const int i = (tid + j * kThreads) * 4;
+        held[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < a.I) held[j] = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
+      }
+      const auto top_of = [](const float4& v) {
+        return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+      };
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, top_of(held[j]));
+      for (int i = (tid + 4 * kThreads) * 4; i < a.I; i += kThreads * 4)
+        top = max(top, top_of(__ldcg(reinterpret_cast<const float4*>(a.h + at + i))));
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) tops[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
+      const float m = clamp_top(top);
+      const RowQuant rq = row_quant<WT>(m);
+      if (tid == 0) a.h_scale[p] = quant_scale<WT>(m) * weight;
+      const auto store = [&](int i, const float4& v) {
+        *reinterpret_cast<unsigned*>(a.hq + at + i) = quantise4<WT>(v.x, v.y, v.z, v.w, rq);
+      };
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((tid + j * kThreads) * 4 < a.I) store((tid + j * kThreads) * 4, held[j]);
+      for (int i = (tid + 4 * kThreads) * 4; i < a.I; i += kThreads * 4)
+        store(i, __ldcg(reinterpret_cast<const float4*>(a.h + at + i)));
+      return;
     }
+    block -= P;
   }
   if (!LORA) return;
-  const int m = matrix_of(a, p);
-  if (m < 0) return;
-  for (int row = warp; row < a.lora.r; row += kWarps) {
-    const __nv_bfloat16* w = a.lora.a2 + ((long long)m * a.lora.r + row) * a.I;
-    float s = 0.f;
-#pragma unroll 4
-    for (int i = lane * 8; i < a.I; i += 256) {
-      const uint4 wv = *reinterpret_cast<const uint4*>(w + i);
-      if (WT == kBf16) {
-        s = dot8(wv, __ldcg(reinterpret_cast<const uint4*>(a.h_hi + at + i)), s);
-        s = dot8(wv, __ldcg(reinterpret_cast<const uint4*>(a.h_lo + at + i)), s);
-      } else {
-        const float4 h0 = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
-        const float4 h1 = __ldcg(reinterpret_cast<const float4*>(a.h + at + i + 4));
-        const unsigned x[4] = {wv.x, wv.y, wv.z, wv.w};
-        const float h[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
+  const int per = (a.lora.r + kWarps - 1) / kWarps;
+  const int p = block / per, row = (block - p * per) * kWarps + warp;
+  const int m = row < a.lora.r && slot_of(a, p) >= 0 ? matrix_of(a, p) : -1;
+  constexpr int kHeld = 8;                       // rows of up to 2048 are read ahead
+  uint4 w[kHeld];
+  float factor = 0.f;
+  const __nv_bfloat16* from = a.lora.a2 + ((long long)max(m, 0) * a.lora.r + row) * a.I;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s = fmaf(__uint_as_float(x[j] << 16), h[2 * j], s);
-          s = fmaf(__uint_as_float(x[j] & 0xffff0000u), h[2 * j + 1], s);
-        }
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = lane * 8 + j * 256;
+    w[j] = make_uint4(0, 0, 0, 0);
+    if (m >= 0 && i < a.I) w[j] = *reinterpret_cast<const uint4*>(from + i);
+  }
+  // bf16 weights: h already carries the routing weight
+  if (m >= 0) factor = a.lora.scaling[m / a.lora.E] * (WT == kBf16 ? 1.f : a.weights[p]);
+  grid_dependency_wait();
+  if (m < 0) return;
+  const size_t at = (size_t)p * a.I;
+  float s = 0.f;
+  const auto add = [&](const uint4& wv, int i) {
+    if (WT == kBf16) {
+      s = dot8(wv, __ldcg(reinterpret_cast<const uint4*>(a.h_hi + at + i)), s);
+      s = dot8(wv, __ldcg(reinterpret_cast<const uint4*>(a.h_lo + at + i)), s);
+    } else {
+      const float4 h0 = __ldcg(reinterpret_cast<const float4*>(a.h + at + i));
+      const float4 h1 = __ldcg(reinterpret_cast<const float4*>(a.h + at + i + 4));
+      const unsigned x[4] = {wv.x, wv.y, wv.z, wv.w};
+      const float h[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s = fmaf(low_bf16(x[j]), h[2 * j], s);
+        s = fmaf(high_bf16(x[j]), h[2 * j + 1], s);
       }
     }
+  };
 #pragma unroll
-    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (lane == 0) {
-      const size_t to = (size_t)p * a.lora.r + row;
-      // bf16 weights: h already carries the routing weight
-      s *= a.lora.scaling[m / a.lora.E] * (WT == kBf16 ? 1.f : a.weights[p]);
-      split(s, a.v_hi + to, a.v_lo + to);
-    }
+  for (int j = 0; j < kHeld; ++j)
+    if (lane * 8 + j * 256 < a.I) add(w[j], lane * 8 + j * 256);
+  for (int i = lane * 8 + kHeld * 256; i < a.I; i += 256)
+    add(*reinterpret_cast<const uint4*>(from + i), i);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  if (lane == 0) {
+    const size_t to = (size_t)p * a.lora.r + row;
+    split(s * factor, a.v_hi + to, a.v_lo + to);
   }
 }
 
@@ -1031,7 +1121,7 @@ __device__ __forceinline__ int tile_rows(int row, int r1) {
 // Chunks per block: where the other operand comes from global memory, two blocks of it have
 // to fit the registers.
 template <int WT, int NT, bool HS>
-constexpr int kDownBlock = HS ? HSKB : WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
+constexpr int kDownBlock = HS ? 4 : WT == kBf16 ? 4 / NT : NT == 4 ? 2 : 4;
 
 // h in shared memory (HS): a row of `stride` bytes (an odd number of 64: lanes of two rows
 // then read all banks) for each pair's h, two for its high and low parts, zeros past a row's
@@ -1054,9 +1144,6 @@ __host__ __device__ inline size_t h_bytes(int P, int I, int rows, int r, int wty
 // Rows that down quantises itself: few enough that every CTA doing so costs less than a
 // launch in between.
 constexpr int kSelfWidth = 1024, kSelfValues = 16384;
-__host__ __device__ inline bool quantises_itself(int P, int I) {
-  return I <= kSelfWidth && P * I <= kSelfValues;
-}
 
 // Whole CTA; ends with a barrier, all earlier copies landed.
 template <int WT, bool LORA>
@@ -1066,7 +1153,7 @@ __device__ void stage_h(const ExpertsArgs& a, const Routing& rt, unsigned char* 
   const int stride = h_stride(a.I, WT), parts = WT == kBf16 ? 2 : 1;
   if (LORA) {              // rows [2p] high, [2p + 1] low parts of v
     const int per = a.lora.r / 8;
-    for (int i = tid; i < P * 2 * per; i += kThreads) {
+    for (int i = tid; i < P * 2 * per; i += blockDim.x) {
       const int row = i / per, at = (i - row * per) * 8, p = row >> 1;
       if (rt.pair_slot[p] < 0 || rt.matrix[p] < 0) continue;
       copy16((unsigned)__cvta_generic_to_shared(v + (size_t)row * a.lora.r + at),
@@ -1075,10 +1162,10 @@ __device__ void stage_h(const ExpertsArgs& a, const Routing& rt, unsigned char* 
     }
     copy_commit();
   }
-  for (int i = tid * 16; i < stride * parts; i += kThreads * 16)
+  for (int i = tid * 16; i < stride * parts; i += blockDim.x * 16)
     *reinterpret_cast<uint4*>(hs + (size_t)P * parts * stride + i) = make_uint4(0, 0, 0, 0);
-  if (WT != kBf16 && quantises_itself(P, a.I)) {
-    for (int p = warp; p < P; p += kWarps) {
+  if (WT != kBf16 && a.self_h) {
+    for (int p = warp; p < P; p += blockDim.x >> 5) {
       if (rt.pair_slot[p] < 0) continue;
       float4 x[kSelfWidth / 128];
       unsigned top = 0;
@@ -1105,7 +1192,7 @@ __device__ void stage_h(const ExpertsArgs& a, const Routing& rt, unsigned char* 
     }
   } else {
     const int row_bytes = a.I * Kind<WT>::kItem, per = (stride - 64) / 16;
-    for (int i = tid; i < P * parts * per; i += kThreads) {
+    for (int i = tid; i < P * parts * per; i += blockDim.x) {
       const int row = i / per, at = (i - row * per) * 16, p = row / parts;
       if (rt.pair_slot[p] < 0) continue;
       const uint8_t* src = WT == kBf16 ? reinterpret_cast<const uint8_t*>(row & 1 ? a.h_lo : a.h_hi)
@@ -1115,29 +1202,33 @@ __device__ void stage_h(const ExpertsArgs& a, const Routing& rt, unsigned char* 
     }
     copy_commit();
     if (WT != kBf16)
-      for (int p = tid; p < P; p += kThreads)
+      for (int p = tid; p < P; p += blockDim.x)
         if (rt.pair_slot[p] >= 0) scale[p] = __ldcg(a.h_scale + p);
   }
   copy_wait<0>();
   __syncthreads();
 }
 
+constexpr int kDownMaxThreads = 512;          // (see alone_threads)
+
 template <int NT>
 constexpr int kRed = kWarps * 16 * 8 * NT;   // the warps' partial sums
 
 template <int WT, int NT, bool LORA, bool HS>
-__global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant__ ExpertsArgs a) {
+__global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
+    down_kernel(const __grid_constant__ ExpertsArgs a) {
   using K = Kind<WT>;
   using Acc = typename K::Acc;
   constexpr int KB = kDownBlock<WT, NT, HS>, kParts = WT == kBf16 ? 2 : 1;
-  using Stream = Fifo<KB, kDownChunks / KB>;
+  using Stream = Fifo<KB, kDownChunks[HS] / KB>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
   const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
   const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x), rows = r1 - r0;
   Stream fifo(smem);
-  const Routing rt = routing_at(smem + kDownFifo, P, NT);
-  float* red = reinterpret_cast<float*>(smem + kDownFifo + routing_bytes(P, NT, LORA));
+  constexpr int kFifo = Stream::kStages * Stream::kStage;
+  const Routing rt = routing_at(smem + kFifo, P, NT);
+  float* red = reinterpret_cast<float*>(smem + kFifo + routing_bytes(P, NT, LORA));
   unsigned char* hs = reinterpret_cast<unsigned char*>(red + kRed<NT>);        // HS
   const int stride = h_stride(a.I, WT);
   unsigned char* after_h = hs + (size_t)(P + 1) * kParts * stride;
@@ -1150,7 +1241,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
   // starts once every CTA of the kernels before it has started, the first of them after its
   // own wait.
   release_dependents();
-  build_routing<NT, LORA>(a, rt, reinterpret_cast<int*>(smem));
+  const FirstReads first(a);
+  build_routing<NT, LORA>(a, rt, first, reinterpret_cast<int*>(smem));
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int row_bytes = a.I * K::kItem, lora_bytes = LORA ? a.lora.r * 2 : 0;
@@ -1160,7 +1252,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
   const int U = units.all();
 
   // The head of the stream: a block of unit hu of the tile at hrow.
-  int hrow = warp < U ? r0 : r1, hn = tile_rows(r0, r1), hu = warp, hb = 0, hend = 0;
+  int hrow = warp < kWarps && warp < U ? r0 : r1, hn = tile_rows(r0, r1), hu = warp, hb = 0, hend = 0;
   int size_a = 0, size_b = 0, hbytes = 0;
   const uint8_t* src = nullptr;
   const auto head_at = [&]() {
@@ -1206,7 +1298,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
   for (int i = 0; i < Stream::kStages; ++i) push();
   if (HS && WT != kBf16) {
     const int n = rt.entries[0] * rows;
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += blockDim.x) {
       const int e = i / rows;
       row_scale[i] = a.s2[(long long)rt.slot[e] * a.H + r0 + (i - e * rows)];
     }
@@ -1218,10 +1310,10 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
   for (int row = r0, n; row < r1; row += n) {
     n = tile_rows(row, r1);
     float acc[NT][4] = {};
-    for (int u = warp; u < U; u += kWarps) {
+    for (int u = warp < kWarps ? warp : U; u < U; u += kWarps) {
       if (LORA && u >= units.units) {
         // an adapted pair: B2's rows with v in its token's column
-        const int p = rt.list[u - units.units], t = p / a.k;
+        const int p = rt.list[u - units.units], t = token_of(a, p);
         const uint4 zero = make_uint4(0, 0, 0, 0);
         for (int at = 0; at < lora_bytes; at += KB * 64) {
           const unsigned f = fifo.front();
@@ -1301,7 +1393,9 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
         }
       };
       if (!HS) fetch(b);
-      Acc sum[NT][4] = {};
+      // (one column tile: two chains of products, as each waits for the one before it)
+      constexpr int kChains = NT == 1 ? 2 : 1;
+      Acc sum[kChains][NT][4] = {};
       for (; b < end; ++b) {
         uint4 now[HS ? 1 : NT][HS ? 1 : KB][HS ? 1 : kParts];
         if (!HS) {
@@ -1332,9 +1426,10 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
               uint4 v;
               if constexpr (HS) v = *reinterpret_cast<const uint4*>(from[nt] + part * stride + j * 64);
               else v = now[nt][j][part];
-              if constexpr (WT == kBf16) chunk_mma_bf16(acc[nt], wa[j], wb[j], v);
-              if constexpr (WT == kInt8) chunk_mma_s8(sum[nt], wa[j], wb[j], v);
-              if constexpr (WT == kFp8) chunk_mma_fp8(sum[nt], fa, fb, v);
+              Acc(&c)[4] = sum[j % kChains][nt];
+              if constexpr (WT == kBf16) chunk_mma_bf16(c, wa[j], wb[j], v);
+              if constexpr (WT == kInt8) chunk_mma_s8(c, wa[j], wb[j], v);
+              if constexpr (WT == kFp8) chunk_mma_fp8(c, fa, fb, v);
             }
           }
         }
@@ -1344,20 +1439,21 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
             if (has[nt]) from[nt] += KB * 64;
         push();
       }
-      if (WT != kBf16) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (NT > 1 && !(mask >> nt & 1)) continue;
-          acc[nt][0] += (float)sum[nt][0] * (rf[0] * cf[nt][0]);
-          acc[nt][1] += (float)sum[nt][1] * (rf[0] * cf[nt][1]);
-          acc[nt][2] += (float)sum[nt][2] * (rf[1] * cf[nt][0]);
-          acc[nt][3] += (float)sum[nt][3] * (rf[1] * cf[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) {
+        if (NT > 1 && !(mask >> nt & 1)) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          Acc v = sum[0][nt][i];
+          if (kChains == 2) v += sum[kChains - 1][nt][i];
+          acc[nt][i] += WT == kBf16 ? (float)v : (float)v * (rf[i >> 1] * cf[nt][i & 1]);
         }
       }
     }
     float* mine = red + warp * 16 * 8 * NT;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      if (warp >= kWarps) break;
       const int col = nt * 8 + 2 * q;
       mine[g * 8 * NT + col] = acc[nt][0];
       mine[g * 8 * NT + col + 1] = acc[nt][1];
@@ -1365,7 +1461,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const __grid_constant
       mine[(g + 8) * 8 * NT + col + 1] = acc[nt][3];
     }
     __syncthreads();
-    for (int o = tid; o < 16 * a.T; o += kThreads) {
+    for (int o = tid; o < 16 * a.T; o += blockDim.x) {
       const int i = o & 15, t = o >> 4;
       if (i >= n) continue;
       float s = 0.f;
@@ -1522,6 +1618,11 @@ cudaError_t allow_smem(Kernel fn, std::atomic<bool>* done, int dev) {
   if (err != cudaSuccess) return err;
   err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              optin - (int)fa.sharedSizeBytes);
+  // An SM is not repartitioned while a CTA is on it: without this the partition that up needs
+  // keeps down off the SM until up has left.
+  if (err == cudaSuccess)
+    err = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
   if (err == cudaSuccess) done[dev].store(true, std::memory_order_release);
   return err;
 }
@@ -1542,6 +1643,27 @@ int launch(void (*fn)(Params...), dim3 grid, int threads, size_t smem, cudaStrea
   return (int)cudaLaunchKernelEx(&cfg, fn, Params(args)...);
 }
 
+// An SM takes one CTA of up and one of down, and not two of a kind (two on one SM and none on
+// another was 25 us to 18 for one token in bf16): two of up do not fit its shared memory, two
+// of down not its registers, for which down is launched with idle warps beside its kWarps
+// (they help to stage h).
+constexpr size_t kUpAlone = (228 * 1024) / 2 - 1024 + 16;
+
+template <typename Kernel>
+int alone_threads(Kernel fn, std::atomic<int>& known, int* threads) {
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaFuncAttributes fa{};
+    const cudaError_t err = cudaFuncGetAttributes(&fa, fn);
+    if (err != cudaSuccess) return (int)err;
+    n = (32768 / ((fa.numRegs + 7) / 8 * 8) / 32 + 1) * 32;
+    n = n < kThreads ? kThreads : n > kDownMaxThreads ? kDownMaxThreads : n;
+    known.store(n, std::memory_order_relaxed);
+  }
+  *threads = n;
+  return 0;
+}
+
 int chunk_columns(int wtype) { return wtype == kBf16 ? 32 : 64; }
 
 size_t staged_bytes(int T, int H, int wtype) {
@@ -1555,8 +1677,8 @@ int column_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : 4; }
 size_t up_bytes(int P, int NT, bool lora) {
   return kUpFifo + routing_bytes(P, NT, lora) + kMaxTokens * 4;
 }
-size_t down_bytes(int P, int NT, bool lora) {
-  return kDownFifo + routing_bytes(P, NT, lora) + (size_t)kWarps * 16 * 8 * NT * 4;
+size_t down_bytes(int P, int NT, bool lora, bool hs) {
+  return down_fifo(hs) + routing_bytes(P, NT, lora) + (size_t)kWarps * 16 * 8 * NT * 4;
 }
 
 // Does the copy of x fit beside it?  bf16 rows are read from L1 / L2 where it does not.
@@ -1607,8 +1729,9 @@ size_t carve(ExpertsArgs* a, unsigned char* base, int tokens, int k, int H, int 
 }
 
 template <int WT, int NT, bool LORA>
-int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
+int run_layer(ExpertsArgs a, cudaStream_t stream) {
   static std::atomic<bool> done_up[2][kMaxDevices], done_down[2][kMaxDevices];
+  static std::atomic<int> alone[kMaxDevices];
   int dev = 0, sms = 0;
   int rc = device_sms(&dev, &sms);
   if (rc != 0) return rc;
@@ -1617,10 +1740,10 @@ int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
   const auto up = staged ? up_kernel<WT, NT, LORA, true> : up_kernel<WT, NT, LORA, WT != kBf16>;
   cudaError_t err = allow_smem(up, done_up[staged], dev);
   const int P = a.T * a.k;
-  size_t down_smem = down_bytes(P, NT, LORA);
-  const size_t in_smem = h_bytes(P, a.I, (a.H + sms - 1) / sms, a.lora.r, WT);
-  const bool hs = down_smem + in_smem <= kSmem;
-  if (hs) down_smem += in_smem;
+  size_t down_smem = down_bytes(P, NT, LORA, true) + h_bytes(P, a.I, (a.H + sms - 1) / sms, a.lora.r, WT);
+  const bool hs = down_smem <= kSmem;
+  a.self_h = WT != kBf16 && hs && a.I <= kSelfWidth && P * a.I <= kSelfValues;
+  if (!hs) down_smem = down_bytes(P, NT, LORA, false);
   const auto down = hs ? down_kernel<WT, NT, LORA, true> : down_kernel<WT, NT, LORA, false>;
   if (err == cudaSuccess) err = allow_smem(down, done_down[hs], dev);
   if (err != cudaSuccess) return (int)err;
@@ -1631,13 +1754,21 @@ int run_layer(const ExpertsArgs& a, cudaStream_t stream) {
     if (rc != 0) return rc;
   }
   rc = launch(up, dim3(sms), kThreads,
-              up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0), stream, a);
+              max(kUpAlone, up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0)),
+              stream, a);
   if (rc != 0) return rc;
-  if (LORA || (WT != kBf16 && !(hs && quantises_itself(P, a.I)))) {
-    rc = launch(mid_kernel<WT, LORA>, dim3(P), kThreads, 0, stream, a);
+  const bool quantise = WT != kBf16 && !a.self_h;
+  if (LORA || quantise) {
+    const int grid = (quantise ? P : 0) + (LORA ? P * ((a.lora.r + kWarps - 1) / kWarps) : 0);
+    rc = launch(mid_kernel<WT, LORA>, dim3(grid), kThreads, 0, stream, a);
     if (rc != 0) return rc;
   }
-  return launch(down, dim3(sms), kThreads, down_smem, stream, a);
+  int threads = kThreads;
+  if (hs && NT < 4) {
+    rc = alone_threads(down, alone[dev], &threads);
+    if (rc != 0) return rc;
+  }
+  return launch(down, dim3(sms), threads, down_smem, stream, a);
 }
 
 template <int WT, bool LORA>
@@ -1717,6 +1848,7 @@ ExpertsArgs experts_args(const void* x, int T, int ldx, int H, const int* ids,
   a.ldo = ldo;
   a.T = T;
   a.k = k;
+  a.per_k = k > 0 ? 1.f / (float)k : 0.f;
   a.H = H;
   a.I = I;
   a.S = S;
