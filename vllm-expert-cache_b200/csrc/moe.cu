@@ -583,8 +583,9 @@ struct HeldX {
     const int per = a.H / 8;
 #pragma unroll
     for (int j = 0; j < kSelfXVectors; ++j) {
-      const int i = threadIdx.x + j * kThreads, t = i / per;
       v[j] = make_uint4(0, 0, 0, 0);
+      if (j * kThreads >= per * a.T) continue;
+      const int i = threadIdx.x + j * kThreads, t = i / per;
       if (t < a.T) v[j] = *reinterpret_cast<const uint4*>(a.x + t * a.ldx + (i - t * per) * 8);
     }
   }
@@ -618,6 +619,8 @@ __device__ void stage_held(const ExpertsArgs& a, const HeldX& x, unsigned char* 
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSelfXVectors; ++j) {
+    // (code that is not run is not fetched: skipping the empty vectors saves 1 us)
+    if (j * kThreads >= per * a.T) break;
     const int t = (tid + j * kThreads) / per;
     const unsigned top = top_bits(x.v[j]);
     if (__all_sync(0xffffffffu, t == __shfl_sync(0xffffffffu, t, 0))) {
@@ -637,6 +640,7 @@ __device__ void stage_held(const ExpertsArgs& a, const HeldX& x, unsigned char* 
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSelfXVectors; ++j) {
+    if (j * kThreads >= per * a.T) break;
     const int i = tid + j * kThreads, t = i / per;
     if (t < a.T)
       *reinterpret_cast<uint2*>(st + staged_byte(a.T, t, (i - t * per) * 8)) =
@@ -848,7 +852,11 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   for (int i = 0; i < Stream::kStages; ++i) push();
 
   if (WT != kBf16 && !a.prepared) stage_held<WT>(a, held, st, xs);
-  if (after_prep) grid_dependency_wait();
+  // The adapters' u is needed at a tile's end only: unless x comes from prep too, each warp
+  // waits for it there.
+  bool waited = true;
+  if (WT != kBf16 && a.prepared) grid_dependency_wait();
+  else waited = !LORA;
   if (WT != kBf16 && a.prepared) {
     stage_rows(a.xq, a.H, a.H, a.T, st);
     copy_commit();
@@ -884,6 +892,21 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       sg = a.s13[(long long)slot * 2 * a.I + r];
       su = a.s13[(long long)slot * 2 * a.I + a.I + r];
     }
+    // u of an adapted column's first chunk (gate's high and low parts, up's), read ahead
+    unsigned cols = LORA ? rt.adapted[tile.e] : 0;
+    uint4 u[LORA ? 4 : 1];
+    const auto read_u = [&](int t, int at, uint4(&to)[LORA ? 4 : 1]) {
+      if constexpr (LORA) {
+        const bool has = g == (t & 7) && at + q * 16 < lora_bytes;
+        const size_t m = (size_t)col[t] * 2 * a.lora.r + q * 8 + at / 2;
+        to[0] = load_or_zero(a.u_hi + m, has);
+        to[1] = load_or_zero(a.u_lo + m, has);
+        to[2] = load_or_zero(a.u_hi + m + a.lora.r, has);
+        to[3] = load_or_zero(a.u_lo + m + a.lora.r, has);
+      }
+    };
+    const bool ahead = waited;
+    if (LORA && ahead && cols) read_u(__ffs(cols) - 1, 0, u);
     Acc acc[NT][4] = {};
     for (int at = 0, blk = 0; at < row_bytes; at += KB * 64) {
       const unsigned f = fifo.front();
@@ -920,21 +943,29 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
     // Adapters: one more product for each adapted column, B13's rows with u in that column
     // alone.  Gate and up have different u, so each takes its half of the 16 rows.
     float add[LORA ? NT : 1][4] = {};
-    if (LORA) {
+    if constexpr (LORA) {
       const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (unsigned cols = rt.adapted[tile.e]; cols; cols &= cols - 1) {
+      if (cols && !waited) {
+        grid_dependency_wait();
+        waited = true;
+      }
+      if (cols && !ahead) read_u(__ffs(cols) - 1, 0, u);
+      for (; cols; cols &= cols - 1) {
         const int t = __ffs(cols) - 1;
-        const size_t up = (size_t)col[t] * 2 * a.lora.r + q * 8;
+        const unsigned rest = cols & (cols - 1);
         for (int at = 0; at < lora_bytes; at += KB * 64) {
           const unsigned f = fifo.front();
 #pragma unroll
           for (int j = 0; j < KB; ++j) {
             if (at + j * 64 >= lora_bytes) break;
-            const bool has = g == (t & 7) && at + j * 64 + q * 16 < lora_bytes;
-            const size_t m = up + at / 2 + j * 32;
-            const uint4 v[4] = {load_or_zero(a.u_hi + m, has), load_or_zero(a.u_lo + m, has),
-                                load_or_zero(a.u_hi + m + a.lora.r, has),
-                                load_or_zero(a.u_lo + m + a.lora.r, has)};
+            uint4 v[4];
+            if (j == 0 && at == 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] = u[i];
+              if (rest) read_u(__ffs(rest) - 1, 0, u);
+            } else {
+              read_u(t, at + j * 64, v);
+            }
             const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -975,6 +1006,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       }
     }
   }
+  if (!waited) grid_dependency_wait();     // this grid's end means prep's, too
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1184,6 +1216,7 @@ __device__ void stage_h(const ExpertsArgs& a, const Routing& rt, unsigned char* 
 #pragma unroll
       for (int j = 0; j < kSelfWidth / 128; ++j) {
         const int i = j * 128 + lane * 4;
+        if (j * 128 >= stride - 64) break;
         if (i < stride - 64)
           *reinterpret_cast<unsigned*>(hs + (size_t)p * stride + i) =
               i < a.I ? quantise4<WT>(x[j].x, x[j].y, x[j].z, x[j].w, rq) : 0;
