@@ -422,3 +422,20 @@ def test_route_then_experts_captured(moe):
         torch.cuda.synchronize()
         check_route((w, ids), moe_ref.route(x, gate, k))
         check(out, *moe_ref.experts(x, w, ids, w13, w2, s13, s2))
+
+
+def test_route_subnormal_and_tiny_operands(moe):
+    """Operands at the bottom of the type's range still order the experts."""
+    g = gen(45)
+    gate = normal(g, 24, 512)
+    x = normal(g, 5, 512)
+    x[0] *= 2.0 ** -130                             # subnormal
+    x[1] *= 2.0 ** -120
+    x[2, ::2] = 2.0 ** -133                         # the smallest subnormal among ordinary ones
+    x[3] = 0
+    x[3, 7] = 2.0 ** -133
+    check_route(moe.route(x, gate, 24), moe_ref.route(x, gate, 24))
+    gate[5] *= 2.0 ** -128                          # and in the router's weight
+    gate[9] = 0
+    gate[9, 3] = 2.0 ** -133
+    check_route(moe.route(x, gate, 24), moe_ref.route(x, gate, 24))

@@ -1507,10 +1507,22 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------
-// route: one CTA per token.  Scores are sums in 64 bits of exact products, so which expert
-// is the k-th best does not hang on the order of a sum.
+// route: a cluster of CTAs takes TT tokens.  Each CTA scores its share of the experts, a warp
+// two at a time, straight from the router's weight; the scores meet in the first CTA's shared
+// memory, where a warp per token picks.  One launch, bound by latency: reading x and the
+// weight, summing, k dependent choices.
+//
+// Scores are sums in 64 bits of exact products, so which expert is the k-th best does not
+// hang on the order of a sum.  A bf16 becomes a double by moving its bits: shifted by 3 into
+// a double's high word, its exponent reads as e - 896 (subnormals included).  x is brought
+// back to its own exponent, the weights are not: sums are multiplied by 2^896 at the end,
+// which is exact.  (The conversion instruction is slower than the 64-bit products.)  A sum is done
+// again with plain conversions where the move does not hold: with an infinity or a NaN among
+// its operands, a subnormal in x, or a result so small that products may have underflowed.
 
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 256, kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteCluster = 8;
+constexpr int kRouteUnroll = 4;
 
 struct RouteArgs {
   const __nv_bfloat16 *x, *gate;
@@ -1522,100 +1534,234 @@ struct RouteArgs {
   float scale;
 };
 
+// The bf16 in the high half of `u` times 2^-896.
+__device__ __forceinline__ double moved(unsigned u) {
+  return __hiloint2double(((int)u >> 3) & 0x8fffffff, 0);
+}
+// The bf16 in the high half of `u`, normal or zero.
+__device__ __forceinline__ double widened(unsigned u) {
+  const int hi = (((int)u >> 3) & 0x8fffffff) + (896 << 20);
+  return __hiloint2double((u & 0x7f800000u) ? hi : 0, 0);
+}
+
+// One dot product with plain conversions: the warp's.
+__device__ __noinline__ double plain_dot(const __nv_bfloat16* w, const uint8_t* x, int H) {
+  double s = 0.0;
+  for (int i = (threadIdx.x & 31); i < H; i += 32)
+    s += (double)__bfloat162float(w[i]) *
+         (double)__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  return s;
+}
+
+__device__ __forceinline__ unsigned remote_shared(const void* p, int rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(r)
+      : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void store_remote(unsigned at, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory");
+}
+
+template <int TT>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  double* score = reinterpret_cast<double*>(smem);           // selection key
-  __shared__ double r_val[kRouteThreads / 32];
-  __shared__ int r_idx[kRouteThreads / 32];
-  __shared__ double s_sum, s_max;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = (a.H * 2 + 15) / 16 * 16;
+  uint8_t* xs = smem;                                              // [TT][row]
+  double* score = reinterpret_cast<double*>(smem + TT * row);      // [TT][E], first CTA
+  unsigned long long* key = reinterpret_cast<unsigned long long*>(score + TT * a.E);   // likewise
+  __shared__ int odd[TT], some[TT];       // x has an inf, a NaN or a subnormal; x is not all zeros
+  const int rank = blockIdx.x % kRouteCluster, t0 = blockIdx.x / kRouteCluster * TT;
+  const int n = min(TT, a.T - t0);
+
   grid_dependency_wait();
   release_dependents();
-  const int tok = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int NW = kRouteThreads / 32;
-  const __nv_bfloat16* x = a.x + tok * a.ldx;
-  for (int e = warp; e < a.E; e += NW) {
-    double s = 0.0;
-    for (int i = lane * 8; i < a.H; i += 256) {
-      const uint4 wv = *reinterpret_cast<const uint4*>(a.gate + (long long)e * a.H + i);
-      const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
-      const unsigned ww[4] = {wv.x, wv.y, wv.z, wv.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+
+  // The warp's pairs of experts, kRouteUnroll * 256 columns of each at a step; the next step's
+  // are on their way while one is multiplied, the first ones while x is read.
+  const int share = (a.E + kRouteCluster - 1) / kRouteCluster;
+  const int e0 = rank * share, e1 = min(a.E, e0 + share);
+  constexpr int kStep = 256 * kRouteUnroll;
+  uint4 next[2][kRouteUnroll];
+  const auto fetch = [&](int e, int i0) {
+    const __nv_bfloat16* w = a.gate + (long long)e * a.H + i0 + lane * 8;
+    const int second = e + 1 < e1 ? a.H : 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s += (double)__uint_as_float(ww[j] << 16) * (double)__uint_as_float(xw[j] << 16);
-        s += (double)__uint_as_float(ww[j] & 0xffff0000u) *
-             (double)__uint_as_float(xw[j] & 0xffff0000u);
-      }
+    for (int j = 0; j < kRouteUnroll; ++j) {
+      const bool in = e < e1 && i0 + lane * 8 + j * 256 < a.H;
+      next[0][j] = load_or_zero(w + j * 256, in);
+      next[1][j] = load_or_zero(w + second + j * 256, in);
     }
+  };
+  fetch(e0 + warp * 2, 0);
+  if (tid < TT) odd[tid] = some[tid] = 0;
+  __syncthreads();
 #pragma unroll
-    for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (lane == 0) {
-      if (a.sigmoid) s = 1.0 / (1.0 + exp(-s)) + (a.bias ? (double)a.bias[e] : 0.0);
-      score[e] = s;
+  for (int t = 0; t < TT; ++t) {
+    for (int i = tid * 8; i < a.H; i += kRouteThreads * 8) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (t < n) v = *reinterpret_cast<const uint4*>(a.x + (t0 + t) * a.ldx + i);
+      *reinterpret_cast<uint4*>(xs + t * row + i * 2) = v;
+      const unsigned u[4] = {v.x, v.y, v.z, v.w};
+      bool special = top_bits(v) >= 0x7f800000u;
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        special |= ((u[m] & 0x7f80u) == 0 && (u[m] & 0x7fu)) ||
+                   ((u[m] & 0x7f800000u) == 0 && (u[m] & 0x7f0000u));
+      if (special) odd[t] = 1;
+      if (top_bits(v)) some[t] = 1;
     }
   }
   __syncthreads();
-  if (!a.sigmoid) {
-    double m = -INFINITY;
-    for (int e = tid; e < a.E; e += kRouteThreads) m = fmax(m, score[e]);
-    for (int off = 16; off; off >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, off));
-    if (lane == 0) r_val[warp] = m;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < NW; ++w) m = fmax(m, r_val[w]);
-      s_max = m;
-    }
-    __syncthreads();
-    double sum = 0.0;
-    for (int e = tid; e < a.E; e += kRouteThreads)
-      if (score[e] == score[e]) sum += exp(score[e] - s_max);
-    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) r_val[warp] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < NW; ++w) sum += r_val[w];
-      s_sum = sum;
-    }
-    __syncthreads();
-  }
-  double total = 0.0;
-  double mine = 0.0;       // thread r < k keeps the r-th weight
-  int mine_id = -1;
-  for (int r = 0; r < a.k; ++r) {
-    double bv = -INFINITY;
-    int bi = -1;
-    for (int e = tid; e < a.E; e += kRouteThreads)
-      if (score[e] > bv) { bv = score[e]; bi = e; }
+
+  for (int e = e0 + warp * 2; e < e1; e += kRouteWarps * 2) {
+    const bool two = e + 1 < e1;
+    const __nv_bfloat16* w0 = a.gate + (long long)e * a.H;
+    const __nv_bfloat16* w1 = w0 + (two ? a.H : 0);
+    double acc[2][TT] = {};
+    unsigned top[2] = {0, 0};
+    for (int step = 0; step < a.H; step += kStep) {
+      const int i0 = step + lane * 8;
+      uint4 w[2][kRouteUnroll];
 #pragma unroll
-    for (int off = 16; off; off >>= 1) {
-      const double ov = __shfl_xor_sync(0xffffffffu, bv, off);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, off);
-      if (oi >= 0 && (bi < 0 || ov > bv || (ov == bv && oi < bi))) { bv = ov; bi = oi; }
-    }
-    if (lane == 0) { r_val[warp] = bv; r_idx[warp] = bi; }
-    __syncthreads();
-    if (tid < 32) {
-      bv = -INFINITY; bi = -1;
-      for (int w = 0; w < NW; ++w)
-        if (r_idx[w] >= 0 && (bi < 0 || r_val[w] > bv || (r_val[w] == bv && r_idx[w] < bi))) {
-          bv = r_val[w];
-          bi = r_idx[w];
-        }
-      double wgt = 0.0;
-      if (bi >= 0) {
-        if (a.sigmoid) wgt = bv - (a.bias ? (double)a.bias[bi] : 0.0);
-        else wgt = exp(bv - s_max) / s_sum;
+      for (int j = 0; j < kRouteUnroll; ++j) {
+        w[0][j] = next[0][j];
+        w[1][j] = next[1][j];
       }
-      total += wgt;
-      if (tid == r) { mine = wgt; mine_id = bi; }
-      __syncwarp();
-      if (tid == 0 && bi >= 0) score[bi] = -INFINITY;
+      if (step + kStep < a.H) fetch(e, step + kStep);
+      else fetch(e + kRouteWarps * 2, 0);
+#pragma unroll 1
+      for (int j = 0; j < kRouteUnroll; ++j) {
+        const int i = i0 + j * 256;
+        if (i >= a.H) break;
+        uint4 wv[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          wv[x] = w[x][0];                        // rotated below: one copy of the code
+          top[x] = max(top[x], top_bits(wv[x]));
+#pragma unroll
+          for (int y = 0; y + 1 < kRouteUnroll; ++y) w[x][y] = w[x][y + 1];
+        }
+        uint4 xv[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) xv[t] = *reinterpret_cast<const uint4*>(xs + t * row + i * 2);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const unsigned u[2] = {(&wv[0].x)[m], (&wv[1].x)[m]};
+          const double lo[2] = {moved(u[0] << 16), moved(u[1] << 16)};
+          const double hi[2] = {moved(u[0] & 0xffff0000u), moved(u[1] & 0xffff0000u)};
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+            const unsigned v = (&xv[t].x)[m];
+            const double xl = widened(v << 16), xh = widened(v & 0xffff0000u);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) acc[x][t] = fma(xh, hi[x], fma(xl, lo[x], acc[x][t]));
+          }
+        }
+      }
     }
-    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const bool bad = __any_sync(0xffffffffu, top[x] >= 0x7f800000u);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        double s = acc[x][t];
+#pragma unroll
+        for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        s *= 0x1p896;
+        if (bad || odd[t] || (fabs(s) < 0x1p-64 && some[t]))
+          s = plain_dot(x ? w1 : w0, xs + t * row, a.H);
+        if (lane == 0 && (x == 0 || two))
+          store_remote(remote_shared(score + t * a.E + e + x, 0), s + 0.0);   // -0 becomes 0
+      }
+    }
   }
-  if (tid < a.k) {
-    if (a.renorm && total > 0.0) mine /= total;
-    a.weights[(long long)tok * a.k + tid] = (float)(mine * (double)a.scale);
-    a.ids[(long long)tok * a.k + tid] = mine_id;
+  asm volatile("barrier.cluster.arrive.release.aligned; barrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+  if (rank != 0) return;
+
+  // ---- a warp picks for its token ------------------------------------------------------
+  // What is compared: the value's bits, made to order as unsigned; 0 = not to be picked.
+  for (int i = tid; i < n * a.E; i += kRouteThreads) {
+    double v = score[i];
+    if (a.sigmoid) v = 1.0 / (1.0 + exp(-v)) + (a.bias ? (double)a.bias[i % a.E] : 0.0);
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    const bool never = v != v || v == -INFINITY;
+    key[i] = never ? 0 : b >> 63 ? ~b : b | 1ull << 63;
+  }
+  __syncthreads();
+  if (warp >= n) return;
+  const int tok = t0 + warp;
+  score += warp * a.E;
+  key += warp * a.E;
+  // A lane's best two of its experts; they are looked for again when both are picked.
+  unsigned long long best = 0, second = 0;
+  int best_e = INT_MAX, second_e = INT_MAX;
+  const auto scan = [&]() {
+    best = second = 0;
+    best_e = second_e = INT_MAX;
+    for (int e = lane; e < a.E; e += 32) {             // ascending: the first of equals stays
+      const unsigned long long o = key[e];
+      if (o > best) {
+        second = best;
+        second_e = best_e;
+        best = o;
+        best_e = e;
+      } else if (o > second) {
+        second = o;
+        second_e = e;
+      }
+    }
+  };
+  scan();
+  int mine = -1;                // lane r < k: the r-th pick
+  for (int r = 0; r < a.k; ++r) {
+    const unsigned hi = (unsigned)(best >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
+    const bool in = hi == top_hi;
+    const unsigned lo = in ? (unsigned)best : 0, top_lo = __reduce_max_sync(0xffffffffu, lo);
+    if ((top_hi | top_lo) == 0) break;
+    const int e = (int)__reduce_min_sync(0xffffffffu,
+                                         in && lo == top_lo ? (unsigned)best_e : 0xffffffffu);
+    if (lane == r) mine = e;
+    if ((e & 31) == lane) {
+      key[e] = 0;               // picked
+      best = second;
+      best_e = second_e;
+      second = 0;
+      second_e = INT_MAX;
+      if (best == 0) scan();
+    }
+  }
+  const double s = mine >= 0 ? score[mine] : 0.0;
+  double weight = 0.0;
+  if (a.sigmoid) {
+    if (mine >= 0) weight = 1.0 / (1.0 + exp(-s));
+  } else {
+    // the first pick is the largest; renormalised, the sum over all experts cancels
+    const double top = __shfl_sync(0xffffffffu, s, 0);
+    if (mine >= 0) weight = exp(s - top);
+    if (!a.renorm) {
+      double all = 0.0;
+      for (int e = lane; e < a.E; e += 32)
+        if (score[e] == score[e]) all += exp(score[e] - top);
+#pragma unroll
+      for (int off = 16; off; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+      weight /= all;
+    }
+  }
+  if (a.renorm) {
+    double total = weight;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (total > 0.0) weight /= total;
+  }
+  if (lane < a.k) {
+    a.weights[(long long)tok * a.k + lane] = mine >= 0 ? (float)(weight * (double)a.scale) : 0.f;
+    a.ids[(long long)tok * a.k + lane] = mine;
   }
 }
 
@@ -1662,17 +1808,19 @@ cudaError_t allow_smem(Kernel fn, std::atomic<bool>* done, int dev) {
 
 template <typename... Params, typename... Args>
 int launch(void (*fn)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
-           const Args&... args) {
+           int cluster, const Args&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return (int)cudaLaunchKernelEx(&cfg, fn, Params(args)...);
 }
 
@@ -1783,17 +1931,17 @@ int run_layer(ExpertsArgs a, cudaStream_t stream) {
   if (LORA || a.prepared) {
     const int grid = (a.prepared ? a.T : 0) +
                      (LORA ? P * ((2 * a.lora.r + kWarps - 1) / kWarps) : 0);
-    rc = launch(prep_kernel<WT, LORA>, dim3(grid), kThreads, 0, stream, a);
+    rc = launch(prep_kernel<WT, LORA>, dim3(grid), kThreads, 0, stream, 1, a);
     if (rc != 0) return rc;
   }
   rc = launch(up, dim3(sms), kThreads,
               max(kUpAlone, up_bytes(P, NT, LORA) + (staged ? staged_bytes(a.T, a.H, WT) : 0)),
-              stream, a);
+              stream, 1, a);
   if (rc != 0) return rc;
   const bool quantise = WT != kBf16 && !a.self_h;
   if (LORA || quantise) {
     const int grid = (quantise ? P : 0) + (LORA ? P * ((a.lora.r + kWarps - 1) / kWarps) : 0);
-    rc = launch(mid_kernel<WT, LORA>, dim3(grid), kThreads, 0, stream, a);
+    rc = launch(mid_kernel<WT, LORA>, dim3(grid), kThreads, 0, stream, 1, a);
     if (rc != 0) return rc;
   }
   int threads = kThreads;
@@ -1801,7 +1949,7 @@ int run_layer(ExpertsArgs a, cudaStream_t stream) {
     rc = alone_threads(down, alone[dev], &threads);
     if (rc != 0) return rc;
   }
-  return launch(down, dim3(sms), threads, down_smem, stream, a);
+  return launch(down, dim3(sms), threads, down_smem, stream, 1, a);
 }
 
 template <int WT, bool LORA>
@@ -1816,6 +1964,22 @@ int run_tiles(const ExpertsArgs& a, cudaStream_t stream) {
 template <int WT>
 int run_type(const ExpertsArgs& a, cudaStream_t stream) {
   return a.lora.r ? run_tiles<WT, true>(a, stream) : run_tiles<WT, false>(a, stream);
+}
+
+size_t route_bytes(int TT, int H, int E) {
+  return (size_t)TT * ((H * 2 + 15) / 16 * 16 + 16 * (size_t)E);
+}
+
+template <int TT>
+int run_route(const RouteArgs& a, cudaStream_t stream) {
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0, sms = 0;
+  const int rc = device_sms(&dev, &sms);
+  if (rc != 0) return rc;
+  const cudaError_t err = allow_smem(route_kernel<TT>, done, dev);
+  if (err != cudaSuccess) return (int)err;
+  return launch(route_kernel<TT>, dim3((a.T + TT - 1) / TT * kRouteCluster), kRouteThreads,
+                route_bytes(TT, a.H, a.E), stream, kRouteCluster, a);
 }
 
 bool misaligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
@@ -1967,7 +2131,11 @@ int expert_cache_route(const void* x, int T, int ldx, int H, const void* gate_w,
   a.sigmoid = scoring;
   a.renorm = renormalize != 0;
   a.scale = scale;
-  return launch(route_kernel, dim3(T), kRouteThreads, (size_t)E * 8, stream, a);
+  // Tokens a cluster: enough clusters to fill the SMs before a weight read serves more.
+  int tt = T <= 4 ? 1 : T <= 36 ? 2 : 4;
+  while (tt > 1 && route_bytes(tt, H, E) > kSmem) tt /= 2;
+  return tt == 1 ? run_route<1>(a, stream) : tt == 2 ? run_route<2>(a, stream)
+                                                     : run_route<4>(a, stream);
 }
 
 }  // extern "C"
