@@ -17,6 +17,9 @@ from torch's caching allocator, read nothing back and can be captured into CUDA 
 ``ExpertSlotCache.forward`` runs them as one cached step.  They have no counterpart in the
 reference, which leaves the layer to vLLM's kernels (vllm_expert_cache/cache.py:118-163
 ends with the gathered slots).
+
+A layer's kernels take some 15 us for one token, so a call's checks are written to be cheap:
+plain comparisons, with the message put together only where one fails.
 """
 
 from __future__ import annotations
@@ -35,39 +38,45 @@ MAX_TOPK = 32           # EXPERT_CACHE_EXPERTS_MAX_TOPK
 MAX_DIM = 32768         # EXPERT_CACHE_EXPERTS_MAX_DIM
 MAX_SLOTS = 1024        # EXPERT_CACHE_MAX_SLOTS
 MAX_RANK = 256          # EXPERT_CACHE_LORA_MAX_RANK
+MAX_HIDDEN = 16384      # EXPERT_CACHE_PREGATE_MAX_HIDDEN
+MAX_EXPERTS = 2048      # EXPERT_CACHE_PREGATE_MAX_EXPERTS
+
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+# The current stream's handle without building a Stream object (2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _is(t: torch.Tensor) -> str:
+    return f"{tuple(t.shape)} {t.dtype} on {t.device}"
 
 
-def _on(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, x on {device}")
-
-
-def _rows(x: torch.Tensor, name: str = "x") -> torch.Tensor:
+def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as the kernels read it: bf16 rows of unit inner stride, 16-byte aligned."""
-    _need(x.dim() == 2 and x.dtype == torch.bfloat16,
-          f"{name} must be a 2-D bf16 tensor, not {tuple(x.shape)} {x.dtype}")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.size(1) or x.data_ptr() % 16:
+    if x.dtype is not _BF16 or x.dim() != 2 or not x.is_cuda:
+        raise ValueError(f"x must be a 2-D bf16 tensor on a GPU, not {_is(x)}")
+    row = x.stride(0)
+    if x.stride(1) != 1 or row % 8 or row < x.size(1) or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
     return x
 
 
-def _call(device, fn, *args) -> None:
-    """`fn(*args, stream)` on the current stream of `device`."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call(index: int, fn, *args) -> None:
+    """`fn(*args, stream)` on the current stream of GPU `index`."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"{fn.__name__} failed rc={rc}")
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    # (a tensor of one row or none may carry any stride)
+    return x.stride(0) if x.size(0) > 1 else (x.size(1) + 7) // 8 * 8
 
 
 def route(x: torch.Tensor, gate_w: torch.Tensor, k: int, *, scoring: str = "softmax",
@@ -82,28 +91,37 @@ def route(x: torch.Tensor, gate_w: torch.Tensor, k: int, *, scoring: str = "soft
     ties go to the lower id, so the choice is the same whatever the order of a sum.  NaN
     scores are never picked; a row with fewer than k others ends in id -1, weight 0.
     """
-    _need(scoring in SCORING, f"scoring must be one of {sorted(SCORING)}, not {scoring!r}")
-    _need(x.is_cuda, "x must be on a GPU")
-    _need(gate_w.dim() == 2 and gate_w.dtype == torch.bfloat16 and gate_w.is_contiguous(),
-          "gate_w must be a contiguous 2-D bf16 tensor")
-    _on(x.device, gate_w=gate_w, bias=bias)
+    mode = SCORING.get(scoring)
+    if mode is None:
+        raise ValueError(f"scoring must be one of {sorted(SCORING)}, not {scoring!r}")
     x = _rows(x)
-    (T, H), E = x.shape, gate_w.size(0)
-    _need(gate_w.size(1) == H, f"gate_w has {gate_w.size(1)} columns, x {H}")
-    _need(H % 8 == 0 and 0 < H <= 16384, f"hidden size {H} is not a multiple of 8 in [8, 16384]")
-    _need(0 < E <= 2048, f"{E} experts: 1 to 2048 are supported")
-    _need(1 <= k <= min(E, MAX_TOPK), f"k={k} of {E} experts: 1 to {min(E, MAX_TOPK)}")
-    _need(gate_w.data_ptr() % 16 == 0, "gate_w is not 16-byte aligned")
+    T, H = x.shape
+    index = x.get_device()
+    if gate_w.dim() != 2 or gate_w.dtype is not _BF16 or not gate_w.is_contiguous() \
+            or gate_w.get_device() != index or gate_w.size(1) != H or gate_w.data_ptr() % 16:
+        raise ValueError(f"gate_w must be a contiguous, 16-byte aligned bf16 [E, {H}] tensor "
+                         f"beside x, not {_is(gate_w)}")
+    E = gate_w.size(0)
+    if H % 8 or not 0 < H <= MAX_HIDDEN:
+        raise ValueError(f"hidden size {H} is not a multiple of 8 up to {MAX_HIDDEN}")
+    if not 0 < E <= MAX_EXPERTS:
+        raise ValueError(f"{E} experts: 1 to {MAX_EXPERTS} are supported")
+    if not 1 <= k <= min(E, MAX_TOPK):
+        raise ValueError(f"k={k} of {E} experts: 1 to {min(E, MAX_TOPK)} are supported")
+    at_bias = None
     if bias is not None:
-        _need(scoring == "sigmoid", "a selection bias needs scoring='sigmoid'")
-        _need(bias.shape == (E,) and bias.dtype == torch.float32 and bias.is_contiguous(),
-              f"bias must be a contiguous fp32 [{E}] tensor")
-    weights = torch.empty((T, k), dtype=torch.float32, device=x.device)
-    ids = torch.empty((T, k), dtype=torch.int32, device=x.device)
-    _call(x.device, lib().expert_cache_route, x.data_ptr(), T, x.stride(0), H,
-          gate_w.data_ptr(), E, k, SCORING[scoring], int(renormalize),
-          None if bias is None else bias.data_ptr(), float(scale), weights.data_ptr(),
-          ids.data_ptr())
+        if mode != 1:
+            raise ValueError("a selection bias needs scoring='sigmoid'")
+        if bias.dim() != 1 or bias.size(0) != E or bias.dtype is not _F32 \
+                or not bias.is_contiguous() or bias.get_device() != index:
+            raise ValueError(f"bias must be a contiguous fp32 [{E}] tensor beside x, not "
+                             f"{_is(bias)}")
+        at_bias = bias.data_ptr()
+    weights = x.new_empty((T, k), dtype=_F32)
+    ids = x.new_empty((T, k), dtype=_I32)
+    _call(index, lib().expert_cache_route, x.data_ptr(), T, _row_stride(x), H,
+          gate_w.data_ptr(), E, k, mode, int(renormalize), at_bias, scale,
+          weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
@@ -112,82 +130,92 @@ def workspace_bytes(T: int, k: int, H: int, I: int, wtype: int, r: int = 0) -> i
     """Device workspace of one call (``expert_cache_experts_workspace``)."""
     n = ctypes.c_long()
     rc = lib().expert_cache_experts_workspace(T, k, H, I, wtype, r, ctypes.byref(n))
-    _need(rc == 0, f"unsupported sizes: T={T} k={k} H={H} I={I} wtype={wtype} r={r}")
+    if rc != 0:
+        raise ValueError(f"unsupported sizes: T={T} k={k} H={H} I={I} wtype={wtype} r={r}")
     return n.value
 
 
-def _scale(scale: torch.Tensor | None, S: int, n: int, name: str):
+def _scale(scale: torch.Tensor | None, S: int, n: int, name: str, index: int) -> int:
     if scale is None:
         raise ValueError(f"8-bit weights need {name}")
-    _need(scale.dtype == torch.float32 and scale.is_contiguous()
-          and scale.shape in ((S, n), (S, n, 1)),
-          f"{name} must be contiguous fp32 [{S}, {n}] or [{S}, {n}, 1], not "
-          f"{tuple(scale.shape)} {scale.dtype}")
+    d = scale.dim()
+    if scale.dtype is not _F32 or d < 2 or d > 3 or scale.size(0) != S or scale.size(1) != n \
+            or (d == 3 and scale.size(2) != 1) or not scale.is_contiguous() \
+            or scale.get_device() != index:
+        raise ValueError(f"{name} must be contiguous fp32 [{S}, {n}] or [{S}, {n}, 1] beside "
+                         f"x, not {_is(scale)}")
     return scale.data_ptr()
 
 
-def _layer_args(x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_map):
-    """Checked arguments of both experts entry points up to I; and the tensors that they
-    point into (a converted copy has to live until the launch is enqueued)."""
-    _need(x.is_cuda, "x must be on a GPU")
-    device = x.device
-    _on(device, topk_weights=topk_weights, topk_ids=topk_ids, w13=w13, w2=w2,
-        w13_scale=w13_scale, w2_scale=w2_scale, expert_map=expert_map)
+def _layer(fn, x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_map,
+           adapters=None):
+    """Checks and the call of both experts entry points."""
     x = _rows(x)
     T, H = x.shape
+    index = x.get_device()
     wtype = WEIGHT_TYPES.get(w13.dtype)
-    _need(wtype is not None and w2.dtype == w13.dtype,
-          f"weights must both be bf16, int8 or float8_e4m3fn, not {w13.dtype} and {w2.dtype}")
-    _need(w13.dim() == 3 and w2.dim() == 3, "w13 and w2 must be 3-D")
+    if wtype is None or w2.dtype is not w13.dtype:
+        raise ValueError("w13 and w2 must both be bf16, int8 or float8_e4m3fn, not "
+                         f"{w13.dtype} and {w2.dtype}")
+    if w13.dim() != 3 or w2.dim() != 3:
+        raise ValueError(f"w13 and w2 must be 3-D, not {_is(w13)} and {_is(w2)}")
     S, I = w2.size(0), w2.size(2)
-    _need(w13.shape == (S, 2 * I, H) and w2.shape == (S, H, I),
-          f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} are not [S, 2I, H] and [S, H, I] "
-          f"for H={H}")
-    _need(w13.is_contiguous() and w2.is_contiguous(), "w13 and w2 must be contiguous")
-    _need(not (w13.data_ptr() | w2.data_ptr()) & 15, "w13 and w2 must be 16-byte aligned")
+    if w2.size(1) != H or w13.size(0) != S or w13.size(1) != 2 * I or w13.size(2) != H:
+        raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} are not [S, 2I, H] "
+                         f"and [S, H, I] for H={H}")
+    at13, at2 = w13.data_ptr(), w2.data_ptr()
+    if not w13.is_contiguous() or not w2.is_contiguous() or (at13 | at2) & 15 \
+            or w13.get_device() != index or w2.get_device() != index:
+        raise ValueError("w13 and w2 must be contiguous, 16-byte aligned and beside x on "
+                         f"GPU {index}")
     vec = 16 if wtype else 8
-    _need(H % vec == 0 and I % vec == 0 and 0 < H <= MAX_DIM and 0 < I <= MAX_DIM,
-          f"H={H} and I={I} must be multiples of {vec} up to {MAX_DIM}")
-    _need(0 < S <= MAX_SLOTS, f"{S} slots: 1 to {MAX_SLOTS} are supported")
+    if H % vec or I % vec or not 0 < H <= MAX_DIM or not 0 < I <= MAX_DIM:
+        raise ValueError(f"H={H} and I={I} must be multiples of {vec} up to {MAX_DIM}")
+    if not 0 < S <= MAX_SLOTS:
+        raise ValueError(f"{S} slots: 1 to {MAX_SLOTS} are supported")
     if wtype:
-        s13 = _scale(w13_scale, S, 2 * I, "w13_scale")
-        s2 = _scale(w2_scale, S, H, "w2_scale")
+        s13 = _scale(w13_scale, S, 2 * I, "w13_scale", index)
+        s2 = _scale(w2_scale, S, H, "w2_scale", index)
     else:
-        _need(w13_scale is None and w2_scale is None, "bf16 weights take no scales")
+        if w13_scale is not None or w2_scale is not None:
+            raise ValueError("bf16 weights take no scales")
         s13 = s2 = None
-    _need(topk_ids.dim() == 2 and topk_ids.size(0) == T
-          and topk_ids.dtype in (torch.int32, torch.int64),
-          f"topk_ids must be int32 or int64 [{T}, k], not {tuple(topk_ids.shape)} "
-          f"{topk_ids.dtype}")
-    k = topk_ids.size(1)
-    _need(1 <= k <= MAX_TOPK, f"k={k}: 1 to {MAX_TOPK} are supported")
-    _need(topk_weights.shape == topk_ids.shape and topk_weights.is_floating_point(),
-          f"topk_weights must be floating point [{T}, {k}], not {tuple(topk_weights.shape)} "
-          f"{topk_weights.dtype}")
-    if topk_ids.dtype != torch.int32:
+    ids = topk_ids
+    if ids.dim() != 2 or ids.size(0) != T or ids.get_device() != index \
+            or (ids.dtype is not _I32 and ids.dtype is not _I64):
+        raise ValueError(f"topk_ids must be int32 or int64 [{T}, k] beside x, not {_is(ids)}")
+    k = ids.size(1)
+    if not 1 <= k <= MAX_TOPK:
+        raise ValueError(f"k={k}: 1 to {MAX_TOPK} are supported")
+    weights = topk_weights
+    if weights.dim() != 2 or weights.size(0) != T or weights.size(1) != k \
+            or weights.get_device() != index or not weights.is_floating_point():
+        raise ValueError(f"topk_weights must be floating point [{T}, {k}] beside x, not "
+                         f"{_is(weights)}")
+    if ids.dtype is not _I32:
         # ids outside int32 must stay out of range, not wrap into it
-        topk_ids = topk_ids.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-    if not topk_ids.is_contiguous():
-        topk_ids = topk_ids.contiguous()
-    if topk_weights.dtype != torch.float32 or not topk_weights.is_contiguous():
-        topk_weights = topk_weights.to(torch.float32).contiguous()
+        ids = ids.clamp(-1, 2 ** 31 - 1).to(_I32)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    if weights.dtype is not _F32 or not weights.is_contiguous():
+        weights = weights.to(_F32).contiguous()
+    at_map = n_map = 0
     if expert_map is not None:
-        _need(expert_map.dim() == 1 and expert_map.dtype == torch.int32
-              and expert_map.is_contiguous() and expert_map.numel() > 0,
-              "expert_map must be a contiguous, non-empty int32 vector")
-    args = (x.data_ptr(), T, x.stride(0), H, topk_ids.data_ptr(), topk_weights.data_ptr(), k,
-            None if expert_map is None else expert_map.data_ptr(),
-            0 if expert_map is None else expert_map.numel(), w13.data_ptr(), s13,
-            w2.data_ptr(), s2, wtype, S, I)
-    return args, (x, topk_ids, topk_weights)
-
-
-def _finish(fn, x, args, more, r):
-    T, H, k, wtype, I = x.size(0), x.size(1), args[6], args[13], args[15]
-    out = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
+        n_map = expert_map.numel()
+        if expert_map.dim() != 1 or expert_map.dtype is not _I32 or n_map == 0 \
+                or not expert_map.is_contiguous() or expert_map.get_device() != index:
+            raise ValueError("expert_map must be a contiguous, non-empty int32 vector beside "
+                             f"x, not {_is(expert_map)}")
+        at_map = expert_map.data_ptr()
+    r, more = 0, ()
+    if adapters is not None:
+        r, more = _adapters(T, H, I, index, *adapters)
+    out = x.new_empty((T, H))
     nbytes = workspace_bytes(T, k, H, I, wtype, r)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
-    _call(x.device, fn, *args, *more, out.data_ptr(), H, ws.data_ptr(), nbytes)
+    workspace = x.new_empty((nbytes // 2,))
+    _call(index, fn, x.data_ptr(), T, _row_stride(x), H, ids.data_ptr(), weights.data_ptr(), k,
+          at_map, n_map, at13, s13, at2, s2, wtype, S, I, *more, out.data_ptr(), H,
+          workspace.data_ptr(), nbytes)
     return out
 
 
@@ -204,9 +232,8 @@ def experts(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
     cache's ``table`` with expert ids, the composed map of ``refresh_ep`` with global ids).
     An id or slot out of range adds nothing, so padded rows carry -1 and give zeros.
     """
-    args, keep = _layer_args(x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale,
-                             expert_map)
-    return _finish(lib().expert_cache_experts, keep[0], args, (), 0)
+    return _layer(lib().expert_cache_experts, x, topk_weights, topk_ids, w13, w2, w13_scale,
+                  w2_scale, expert_map)
 
 
 def experts_lora(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
@@ -224,26 +251,31 @@ def experts_lora(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Te
     map an adapter follows its expert through the slots without being moved.  ``scaling``
     is fp32 [L].
     """
-    args, keep = _layer_args(x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale,
-                             expert_map)
-    x = keep[0]
-    T, H, I = x.size(0), x.size(1), args[15]
-    _on(x.device, a13=a13, b13=b13, a2=a2, b2=b2, scaling=scaling, adapter=adapter)
-    _need(a13.dim() == 4 and a2.dim() == 4, "adapter matrices must be 4-D")
+    return _layer(lib().expert_cache_experts_lora, x, topk_weights, topk_ids, w13, w2,
+                  w13_scale, w2_scale, expert_map, (a13, b13, a2, b2, scaling, adapter))
+
+
+def _adapters(T, H, I, index, a13, b13, a2, b2, scaling, adapter):
+    """Rank and arguments of the adapters, checked."""
+    if a13.dim() != 4 or a2.dim() != 4:
+        raise ValueError(f"adapter matrices must be 4-D, not {_is(a13)} and {_is(a2)}")
     L, E, r = a13.size(0), a13.size(1), a2.size(2)
-    _need(L > 0 and E > 0 and r % 8 == 0 and 0 < r <= MAX_RANK,
-          f"L={L} adapters, E={E} experts, rank {r}: the rank must be a multiple of 8 up to "
-          f"{MAX_RANK}")
-    for name, t, shape in (("a13", a13, (L, E, 2 * r, H)), ("b13", b13, (L, E, 2 * I, r)),
-                           ("a2", a2, (L, E, r, I)), ("b2", b2, (L, E, H, r))):
-        _need(t.shape == shape and t.dtype == torch.bfloat16 and t.is_contiguous()
-              and t.data_ptr() % 16 == 0,
-              f"{name} must be contiguous, 16-byte aligned bf16 {shape}, not "
-              f"{tuple(t.shape)} {t.dtype}")
-    _need(scaling.shape == (L,) and scaling.dtype == torch.float32 and scaling.is_contiguous(),
-          f"scaling must be contiguous fp32 [{L}]")
-    _need(adapter.shape == (T,) and adapter.dtype == torch.int32 and adapter.is_contiguous(),
-          f"adapter must be contiguous int32 [{T}]")
-    more = (adapter.data_ptr(), a13.data_ptr(), b13.data_ptr(), a2.data_ptr(), b2.data_ptr(),
-            scaling.data_ptr(), L, E, r)
-    return _finish(lib().expert_cache_experts_lora, x, args, more, r)
+    if L < 1 or E < 1 or r % 8 or not 0 < r <= MAX_RANK:
+        raise ValueError(f"{L} adapters of {E} experts, rank {r}: the rank must be a multiple "
+                         f"of 8 up to {MAX_RANK}")
+    args = []
+    for name, t, rows, cols in (("a13", a13, 2 * r, H), ("b13", b13, 2 * I, r),
+                                ("a2", a2, r, I), ("b2", b2, H, r)):
+        at = t.data_ptr()
+        if t.shape != (L, E, rows, cols) or t.dtype is not _BF16 or at % 16 \
+                or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(f"{name} must be contiguous, 16-byte aligned bf16 "
+                             f"{(L, E, rows, cols)} beside x, not {_is(t)}")
+        args.append(at)
+    if scaling.shape != (L,) or scaling.dtype is not _F32 or not scaling.is_contiguous() \
+            or scaling.get_device() != index:
+        raise ValueError(f"scaling must be contiguous fp32 [{L}] beside x, not {_is(scaling)}")
+    if adapter.shape != (T,) or adapter.dtype is not _I32 or not adapter.is_contiguous() \
+            or adapter.get_device() != index:
+        raise ValueError(f"adapter must be contiguous int32 [{T}] beside x, not {_is(adapter)}")
+    return r, (adapter.data_ptr(), *args, scaling.data_ptr(), L, E, r)
