@@ -31,6 +31,7 @@ import sys
 
 import torch
 
+from .. import moe
 from ..cache import ExpertSlotCache
 from ..config import settings
 
@@ -306,6 +307,69 @@ def _weight_names(layer) -> tuple[str, str] | None:
     return None
 
 
+def _own_kernel_unusable(layer, method, cache: ExpertSlotCache, cfg) -> str | None:
+    """Why expert_cache_experts cannot stand in for this layer's stock kernel, or None.
+
+    It computes SwiGLU experts in vLLM's registered weight layout (gate rows, then up rows),
+    in bf16 or with 8-bit weights of one scale per output row and activations quantised per
+    token, so the stock kernel has to be one that does the same from the same layout, with
+    nothing dispatched to other ranks around it.
+    """
+    kernel = method.moe_kernel
+    if type(kernel.fused_experts).__name__ != "TritonExperts":
+        return f"{type(kernel.fused_experts).__name__} may keep its weights in another layout"
+    around = type(getattr(kernel, "prepare_finalize", None)).__name__
+    if around != "MoEPrepareAndFinalizeNoDPEPModular":
+        return f"{around} moves tokens around the kernel"
+    act = getattr(layer, "activation", None)
+    if getattr(act, "value", act) != "silu":
+        return f"activation {act}"
+    if getattr(layer, "apply_router_weight_on_input", False):
+        return "router weights are applied on the input"
+    w13, w2 = cache.slots.get("w13_weight"), cache.slots.get("w2_weight")
+    if w13 is None or w2 is None or w13.dim() != 3 or w2.dim() != 3:
+        return "no plain w13_weight / w2_weight pair"
+    wtype = moe.WEIGHT_TYPES.get(w13.dtype)
+    S, H, I = w2.shape
+    if wtype is None or w2.dtype != w13.dtype:
+        return f"weights are {w13.dtype} and {w2.dtype}"
+    if tuple(w13.shape) != (S, 2 * I, H):
+        return f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} are not [E, 2I, H], [E, H, I]"
+    vec = 16 if wtype else 8
+    if H % vec or I % vec or max(H, I) > moe.MAX_DIM or S > moe.MAX_SLOTS:
+        return f"hidden {H}, expert width {I} or {S} slots beyond the kernels' limits"
+    want = {"w13_weight", "w2_weight"}
+    if wtype:
+        want |= {"w13_weight_scale", "w2_weight_scale"}
+    if set(cache.names) != want:
+        return "per-expert tensors " + ", ".join(cache.names)
+    if cfg is None:
+        return "no quant config" if wtype else None
+    for name in _QUANT_DESCS:
+        d = getattr(cfg, name, None)
+        if getattr(d, "bias", None) is not None or getattr(d, "zp", None) is not None or \
+                getattr(d, "alpha_or_gscale", None) is not None:
+            return f"{name} has a bias, zero point or global scale"
+    if getattr(cfg, "gemm1_clamp_limit", None) is not None:
+        return "clamped activation"
+    acts = [getattr(getattr(cfg, n, None), "dtype", None) for n in ("_a1", "_a2")]
+    if not wtype:
+        return None if acts == [None, None] else f"activations are {acts[0]}"
+    if acts != [w13.dtype, w13.dtype]:
+        return f"8-bit weights with {acts[0] or 'unquantised'} activations"
+    for name in ("_a1", "_a2"):
+        d = getattr(cfg, name)
+        shape = getattr(d, "shape", None)
+        if getattr(d, "scale", None) is not None or \
+                (getattr(shape, "row", None), getattr(shape, "col", None)) != (1, -1):
+            return f"{name} is not quantised dynamically per token"
+    for name, rows in (("w13", 2 * I), ("w2", H)):
+        sc = cache.slots[name + "_weight_scale"]
+        if sc.dtype != torch.float32 or tuple(sc.shape) not in ((S, rows), (S, rows, 1)):
+            return f"{name} scale {tuple(sc.shape)} {sc.dtype} is not fp32 per output row"
+    return None
+
+
 def arm(layer, method, logger) -> bool:
     """Attach a slot cache to one MoE layer; True when the cache is live."""
     kind = type(method).__name__
@@ -378,6 +442,20 @@ def arm(layer, method, logger) -> bool:
             logger.info("expert-cache: not splitting wide steps of %s -- %s", kind, why)
             split_max = 0
     split = [split_max]
+    own_kernel = False
+    if settings.moe:
+        why = _own_kernel_unusable(layer, method, cache, slot_cfg)
+        own_kernel = why is None
+        if why is not None:
+            logger.info("expert-cache: %s keeps its own kernel -- %s", kind, why)
+
+    def own_step(x, topk_weights, topk_ids, shared_experts) -> bool:
+        return (own_kernel and shared_experts is None and topk_ids.dim() == 2
+                and topk_ids.size(1) <= moe.MAX_TOPK and isinstance(x, torch.Tensor)
+                and x.dim() == 2 and x.dtype == torch.bfloat16
+                and x.size(1) == cache.slots["w2_weight"].size(1)
+                and isinstance(topk_weights, torch.Tensor)
+                and topk_weights.shape == topk_ids.shape)
 
     def cached(layer, x, topk_weights, topk_ids, shared_experts, shared_experts_input,
                fork=True):
@@ -392,12 +470,18 @@ def arm(layer, method, logger) -> bool:
             if fork and cache.next is not None and topk_ids.dim() == 2 and \
                     isinstance(x, torch.Tensor):
                 _fork_prefetch(cache, x, topk_ids.size(1))
+            if own_step(x, topk_weights, topk_ids, shared_experts):
+                layer.global_num_experts = saved[2]
+                return cache.experts(x, topk_weights, topk_ids, cache.table)
         else:
             # Expert parallel: the routing ids stay global; the layer's expert map is
             # replaced by the composed global id -> slot map for this step.
             ids = topk_ids
             full_map = getattr(layer, ep_name)
-            _set_tensor(layer, ep_name, cache.refresh_ep(topk_ids, full_map))
+            slot_map = cache.refresh_ep(topk_ids, full_map)
+            if own_step(x, topk_weights, topk_ids, shared_experts):
+                return cache.experts(x, topk_weights, topk_ids, slot_map)
+            _set_tensor(layer, ep_name, slot_map)
         experts.quant_config = slot_cfg
         method.moe_quant_config = slot_cfg
         try:

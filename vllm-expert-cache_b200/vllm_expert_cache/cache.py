@@ -29,6 +29,7 @@ import ctypes
 
 import torch
 
+from . import moe
 from ._lib import GATHER_SLOTS, STEP_MAX_SLOTS, lib
 from .config import settings
 
@@ -223,6 +224,45 @@ class ExpertSlotCache:
                                     gate_w.size(0), k, _ptr(out), stream)
         if rc != 0:
             raise RuntimeError(f"expert_cache_pregate failed rc={rc}")
+
+    def experts(self, x: torch.Tensor, topk_weights: torch.Tensor, ids: torch.Tensor,
+                expert_map: torch.Tensor, adapters=None,
+                adapter: torch.Tensor | None = None) -> torch.Tensor:
+        """The MoE layer on the slots as they are (``moe.experts`` / ``moe.experts_lora``).
+
+        ``ids`` are looked up in ``expert_map``: expert ids with the cache's own ``table``,
+        or global ids with the map that ``refresh_ep`` returned.  ``adapters`` is
+        ``(a13, b13, a2, b2, scaling)`` with each token's adapter in ``adapter``.
+        """
+        s = self.slots
+        args = (x, topk_weights, ids, s["w13_weight"], s["w2_weight"])
+        scales = {"w13_scale": s.get("w13_weight_scale"),
+                  "w2_scale": s.get("w2_weight_scale"), "expert_map": expert_map}
+        if adapters is None:
+            return moe.experts(*args, **scales)
+        if adapter is None:
+            raise ValueError("adapters need each token's index in `adapter`")
+        return moe.experts_lora(*args, *adapters, adapter, **scales)
+
+    def forward(self, x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
+                expert_map: torch.Tensor | None = None, adapters=None,
+                adapter: torch.Tensor | None = None) -> torch.Tensor:
+        """A whole cached MoE layer: the step (``refresh``, or ``refresh_ep`` where
+        ``expert_map`` is an expert-parallel layer's), then the experts' arithmetic.
+
+        ``topk_ids`` are expert ids (global ones with ``expert_map``); negative ids are
+        batch padding and add nothing.  With ``moe.route`` before it this is the layer from
+        hidden states to output.  A step wider than the slots is refused: unlike a caller
+        with the full weights at hand, the cache cannot serve it.
+        """
+        if not self.fits(topk_ids):
+            raise ValueError(f"{topk_ids.numel()} routed pairs do not fit {self.S} slots")
+        if expert_map is None:
+            self.refresh(topk_ids)
+            expert_map = self.table
+        else:
+            expert_map = self.refresh_ep(topk_ids, expert_map)
+        return self.experts(x, topk_weights, topk_ids, expert_map, adapters, adapter)
 
     def stats(self) -> dict:
         """Host snapshot of the counters (synchronises; call outside the hot path)."""
