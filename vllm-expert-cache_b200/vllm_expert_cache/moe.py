@@ -138,10 +138,8 @@ def workspace_bytes(T: int, k: int, H: int, I: int, wtype: int, r: int = 0) -> i
 def _scale(scale: torch.Tensor | None, S: int, n: int, name: str, index: int) -> int:
     if scale is None:
         raise ValueError(f"8-bit weights need {name}")
-    d = scale.dim()
-    if scale.dtype is not _F32 or d < 2 or d > 3 or scale.size(0) != S or scale.size(1) != n \
-            or (d == 3 and scale.size(2) != 1) or not scale.is_contiguous() \
-            or scale.get_device() != index:
+    if scale.dtype is not _F32 or scale.shape not in ((S, n, 1), (S, n)) \
+            or not scale.is_contiguous() or scale.get_device() != index:
         raise ValueError(f"{name} must be contiguous fp32 [{S}, {n}] or [{S}, {n}, 1] beside "
                          f"x, not {_is(scale)}")
     return scale.data_ptr()
@@ -153,18 +151,19 @@ def _layer(fn, x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_m
     x = _rows(x)
     T, H = x.shape
     index = x.get_device()
-    wtype = WEIGHT_TYPES.get(w13.dtype)
-    if wtype is None or w2.dtype is not w13.dtype:
+    dtype = w13.dtype
+    wtype = WEIGHT_TYPES.get(dtype)
+    if wtype is None or w2.dtype is not dtype:
         raise ValueError("w13 and w2 must both be bf16, int8 or float8_e4m3fn, not "
-                         f"{w13.dtype} and {w2.dtype}")
-    if w13.dim() != 3 or w2.dim() != 3:
+                         f"{dtype} and {w2.dtype}")
+    if w2.dim() != 3:
         raise ValueError(f"w13 and w2 must be 3-D, not {_is(w13)} and {_is(w2)}")
-    S, I = w2.size(0), w2.size(2)
-    if w2.size(1) != H or w13.size(0) != S or w13.size(1) != 2 * I or w13.size(2) != H:
+    S, rows, I = w2.shape
+    if rows != H or w13.shape != (S, 2 * I, H):
         raise ValueError(f"w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} are not [S, 2I, H] "
                          f"and [S, H, I] for H={H}")
     at13, at2 = w13.data_ptr(), w2.data_ptr()
-    if not w13.is_contiguous() or not w2.is_contiguous() or (at13 | at2) & 15 \
+    if (at13 | at2) & 15 or not w13.is_contiguous() or not w2.is_contiguous() \
             or w13.get_device() != index or w2.get_device() != index:
         raise ValueError("w13 and w2 must be contiguous, 16-byte aligned and beside x on "
                          f"GPU {index}")
@@ -180,16 +179,16 @@ def _layer(fn, x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_m
         if w13_scale is not None or w2_scale is not None:
             raise ValueError("bf16 weights take no scales")
         s13 = s2 = None
-    ids = topk_ids
-    if ids.dim() != 2 or ids.size(0) != T or ids.get_device() != index \
-            or (ids.dtype is not _I32 and ids.dtype is not _I64):
+    ids, weights = topk_ids, topk_weights
+    shape = ids.shape
+    if len(shape) != 2 or shape[0] != T or ids.get_device() != index \
+            or ids.dtype not in (_I32, _I64):
         raise ValueError(f"topk_ids must be int32 or int64 [{T}, k] beside x, not {_is(ids)}")
-    k = ids.size(1)
+    k = shape[1]
     if not 1 <= k <= MAX_TOPK:
         raise ValueError(f"k={k}: 1 to {MAX_TOPK} are supported")
-    weights = topk_weights
-    if weights.dim() != 2 or weights.size(0) != T or weights.size(1) != k \
-            or weights.get_device() != index or not weights.is_floating_point():
+    if weights.shape != shape or weights.get_device() != index \
+            or not weights.is_floating_point():
         raise ValueError(f"topk_weights must be floating point [{T}, {k}] beside x, not "
                          f"{_is(weights)}")
     if ids.dtype is not _I32:
@@ -202,7 +201,7 @@ def _layer(fn, x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_m
     at_map = n_map = 0
     if expert_map is not None:
         n_map = expert_map.numel()
-        if expert_map.dim() != 1 or expert_map.dtype is not _I32 or n_map == 0 \
+        if expert_map.dtype is not _I32 or n_map == 0 or expert_map.dim() != 1 \
                 or not expert_map.is_contiguous() or expert_map.get_device() != index:
             raise ValueError("expert_map must be a contiguous, non-empty int32 vector beside "
                              f"x, not {_is(expert_map)}")
@@ -210,12 +209,12 @@ def _layer(fn, x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_m
     r, more = 0, ()
     if adapters is not None:
         r, more = _adapters(T, H, I, index, *adapters)
-    out = x.new_empty((T, H))
     nbytes = workspace_bytes(T, k, H, I, wtype, r)
-    workspace = x.new_empty((nbytes // 2,))
+    out = torch.empty_like(x)              # x's rows are dense or strided: out's are dense
+    workspace = x.new_empty(nbytes // 2)
     _call(index, fn, x.data_ptr(), T, _row_stride(x), H, ids.data_ptr(), weights.data_ptr(), k,
-          at_map, n_map, at13, s13, at2, s2, wtype, S, I, *more, out.data_ptr(), H,
-          workspace.data_ptr(), nbytes)
+          at_map, n_map, at13, s13, at2, s2, wtype, S, I, *more, out.data_ptr(),
+          _row_stride(out), workspace.data_ptr(), nbytes)
     return out
 
 
