@@ -439,3 +439,28 @@ def test_route_subnormal_and_tiny_operands(moe):
     gate[9] = 0
     gate[9, 3] = 2.0 ** -133
     check_route(moe.route(x, gate, 24), moe_ref.route(x, gate, 24))
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+@pytest.mark.parametrize("T,k,S,H,I,L,r", [
+    (16, 4, 10, 2064, 4096, 0, 0), (21, 4, 36, 488, 3184, 2, 8), (32, 8, 40, 160, 1040, 0, 0),
+    (2, 2, 4, 1024, 14336, 0, 0), (13, 8, 8, 736, 3936, 3, 256), (1, 3, 3, 64, 32768, 0, 0)])
+def test_experts_h_in_segments(moe, kind, T, k, S, H, I, L, r):
+    """More of h than the second kernel can hold at once."""
+    g = gen(T + I)
+    vec = 8 if kind == "bf16" else 16
+    H = H // vec * vec
+    w13, w2, s13, s2 = weights_of(g, kind, S, I, H)
+    x = normal(g, T, H)
+    w, ids = routing(g, T, k, S)
+    ids[T // 2, 0] = -1
+    args = dict(w13_scale=s13, w2_scale=s2)
+    if L:
+        lora = adapters_of(g, L, S, r, H, I)
+        adapter = torch.randint(-1, L, (T,), generator=g, device=DEV, dtype=torch.int32)
+        got = moe.experts_lora(x, w, ids, w13, w2, *lora, adapter, **args)
+        check(got, *moe_ref.experts(x, w, ids, w13, w2, s13, s2, None, lora, adapter))
+    else:
+        got = moe.experts(x, w, ids, w13, w2, **args)
+        check(got, *moe_ref.experts(x, w, ids, w13, w2, s13, s2))
+        assert torch.equal(got, moe.experts(x, w, ids, w13, w2, **args))

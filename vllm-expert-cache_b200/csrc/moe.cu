@@ -351,16 +351,24 @@ __device__ __forceinline__ unsigned e4m3x2_to_f16x2(unsigned v) {
   return r;
 }
 
-// acc += (16 rows: a, b) x (8 columns: v) over one chunk.
-__device__ __forceinline__ void chunk_mma_bf16(float (&c)[4], const uint4& a, const uint4& b,
-                                               const uint4& v) {
-  mma_bf16(c, a.x, b.x, a.y, b.y, v.x, v.y);
-  mma_bf16(c, a.z, b.z, a.w, b.w, v.z, v.w);
+// Sums are kept in four parts, each product's after the one before it in another part: a
+// product waits some 20 cycles for its accumulator, and two warps a scheduler do not hide a
+// chain of them (12 tokens of 6 of 9 experts 79 -> 76 us).  In two parts for 8-bit weights and
+// one column tile: the registers of more keep the next CTA off the SM (one token int8
+// 14.2 -> 15.2 us).
+template <int WT, int NT>
+constexpr int kSumParts = WT != kBf16 && NT == 1 ? 2 : 4;
+
+// (16 rows: a, b) x (8 columns: v) over one chunk, added to parts c0 and c1.
+__device__ __forceinline__ void chunk_mma_bf16(float (&c0)[4], float (&c1)[4], const uint4& a,
+                                               const uint4& b, const uint4& v) {
+  mma_bf16(c0, a.x, b.x, a.y, b.y, v.x, v.y);
+  mma_bf16(c1, a.z, b.z, a.w, b.w, v.z, v.w);
 }
-__device__ __forceinline__ void chunk_mma_s8(int (&c)[4], const uint4& a, const uint4& b,
-                                             const uint4& v) {
-  mma_s8(c, a.x, b.x, a.y, b.y, v.x, v.y);
-  mma_s8(c, a.z, b.z, a.w, b.w, v.z, v.w);
+__device__ __forceinline__ void chunk_mma_s8(int (&c0)[4], int (&c1)[4], const uint4& a,
+                                             const uint4& b, const uint4& v) {
+  mma_s8(c0, a.x, b.x, a.y, b.y, v.x, v.y);
+  mma_s8(c1, a.z, b.z, a.w, b.w, v.z, v.w);
 }
 
 // 16 e4m3 values as fp16: lane's words for four m16n8k16 products.
@@ -377,11 +385,22 @@ __device__ __forceinline__ Wide widen(const uint4& v) {
   }
   return w;
 }
-__device__ __forceinline__ void chunk_mma_fp8(float (&c)[4], const Wide& a, const Wide& b,
-                                              const uint4& v) {
+template <int N, int NT>
+__device__ __forceinline__ void chunk_mma_fp8(float (&c)[N][NT][4], int nt, const Wide& a,
+                                              const Wide& b, const uint4& v) {
   const Wide w = widen(v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mma_f16(c, a.lo[i], b.lo[i], a.hi[i], b.hi[i], w.lo[i], w.hi[i]);
+  for (int i = 0; i < 4; ++i)
+    mma_f16(c[i % N][nt], a.lo[i], b.lo[i], a.hi[i], b.hi[i], w.lo[i], w.hi[i]);
+}
+
+// The sum of the parts.
+template <typename Acc, int N, int NT>
+__device__ __forceinline__ Acc whole(const Acc (&c)[N][NT][4], int nt, int i) {
+  Acc s = c[0][nt][i];
+#pragma unroll
+  for (int part = 1; part < N; ++part) s += c[part][nt][i];
+  return s;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -907,7 +926,8 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
     };
     const bool ahead = waited;
     if (LORA && ahead && cols) read_u(__ffs(cols) - 1, 0, u);
-    Acc acc[NT][4] = {};
+    constexpr int kN = kSumParts<WT, NT>;
+    Acc acc[kN][NT][4] = {};
     for (int at = 0, blk = 0; at < row_bytes; at += KB * 64) {
       const unsigned f = fifo.front();
       uint4 wa[KB], wb[KB];
@@ -931,9 +951,11 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
             if (at + j * 64 + q * 16 < row_bytes)
               v = *reinterpret_cast<const uint4*>(xg[nt] + (at + j * 64) / 2);
           }
-          if constexpr (WT == kBf16) chunk_mma_bf16(acc[nt], wa[j], wb[j], v);
-          if constexpr (WT == kInt8) chunk_mma_s8(acc[nt], wa[j], wb[j], v);
-          if constexpr (WT == kFp8) chunk_mma_fp8(acc[nt], fa, fb, v);
+          auto& c0 = acc[2 * j % kN][nt];
+          auto& c1 = acc[(2 * j + 1) % kN][nt];
+          if constexpr (WT == kBf16) chunk_mma_bf16(c0, c1, wa[j], wb[j], v);
+          if constexpr (WT == kInt8) chunk_mma_s8(c0, c1, wa[j], wb[j], v);
+          if constexpr (WT == kFp8) chunk_mma_fp8(acc, nt, fa, fb, v);
         }
       }
       push();      // into the stage just read, whose vectors the products have taken
@@ -972,10 +994,10 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
               // (a product with zeros in the other column tiles: a branch around it would
               // index the accumulators at run time and put them into local memory)
               const bool here = NT == 1 || t >> 3 == nt;
-              chunk_mma_bf16(add[nt], wa, zero, here ? v[0] : zero);
-              chunk_mma_bf16(add[nt], wa, zero, here ? v[1] : zero);
-              chunk_mma_bf16(add[nt], zero, wb, here ? v[2] : zero);
-              chunk_mma_bf16(add[nt], zero, wb, here ? v[3] : zero);
+              chunk_mma_bf16(add[nt], add[nt], wa, zero, here ? v[0] : zero);
+              chunk_mma_bf16(add[nt], add[nt], wa, zero, here ? v[1] : zero);
+              chunk_mma_bf16(add[nt], add[nt], zero, wb, here ? v[2] : zero);
+              chunk_mma_bf16(add[nt], add[nt], zero, wb, here ? v[3] : zero);
             }
           }
           push();
@@ -990,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       for (int j = 0; j < 2; ++j) {
         const int t = nt * 8 + 2 * q + j, p = col[t];
         if (p < 0) continue;
-        float gate = (float)acc[nt][j], up = (float)acc[nt][2 + j];
+        float gate = (float)whole(acc, nt, j), up = (float)whole(acc, nt, 2 + j);
         if (WT != kBf16) {
           gate *= xs[t] * sg;
           up *= xs[t] * su;
@@ -1369,8 +1391,8 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const bool here = NT == 1 || t >> 3 == nt;
-              chunk_mma_bf16(acc[nt], wa, wb, here ? hi : zero);
-              chunk_mma_bf16(acc[nt], wa, wb, here ? lo : zero);
+              chunk_mma_bf16(acc[nt], acc[nt], wa, wb, here ? hi : zero);
+              chunk_mma_bf16(acc[nt], acc[nt], wa, wb, here ? lo : zero);
             }
           }
           push();
@@ -1426,9 +1448,8 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
         }
       };
       if (!HS) fetch(b);
-      // (one column tile: two chains of products, as each waits for the one before it)
-      constexpr int kChains = NT == 1 ? 2 : 1;
-      Acc sum[kChains][NT][4] = {};
+      constexpr int kN = kSumParts<WT, NT>;
+      Acc sum[kN][NT][4] = {};
       for (; b < end; ++b) {
         uint4 now[HS ? 1 : NT][HS ? 1 : KB][HS ? 1 : kParts];
         if (!HS) {
@@ -1459,10 +1480,11 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
               uint4 v;
               if constexpr (HS) v = *reinterpret_cast<const uint4*>(from[nt] + part * stride + j * 64);
               else v = now[nt][j][part];
-              Acc(&c)[4] = sum[j % kChains][nt];
-              if constexpr (WT == kBf16) chunk_mma_bf16(c, wa[j], wb[j], v);
-              if constexpr (WT == kInt8) chunk_mma_s8(c, wa[j], wb[j], v);
-              if constexpr (WT == kFp8) chunk_mma_fp8(c, fa, fb, v);
+              const int c = 2 * (WT == kBf16 ? part : j & 1);
+              if constexpr (WT == kBf16) chunk_mma_bf16(sum[c][nt], sum[c + 1][nt], wa[j], wb[j], v);
+              if constexpr (WT == kInt8)
+                chunk_mma_s8(sum[c % kN][nt], sum[(c + 1) % kN][nt], wa[j], wb[j], v);
+              if constexpr (WT == kFp8) chunk_mma_fp8(sum, nt, fa, fb, v);
             }
           }
         }
@@ -1477,8 +1499,7 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
         if (NT > 1 && !(mask >> nt & 1)) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          Acc v = sum[0][nt][i];
-          if (kChains == 2) v += sum[kChains - 1][nt][i];
+          const Acc v = whole(sum, nt, i);
           acc[nt][i] += WT == kBf16 ? (float)v : (float)v * (rf[i >> 1] * cf[nt][i & 1]);
         }
       }
