@@ -9,23 +9,39 @@
 // Each routed expert's weights are read once, 3*H*I elements for a handful of tokens: the
 // layer is bound by those bytes, so everything else is arranged around streaming them.
 //
-//   up_kernel     [G; U] and h.  The routed slots' rows are one flat range, split evenly
-//                 over the CTAs.  A tile is 8 (gate, up) row pairs: as the 16 rows of an
-//                 m16n8k16 product they leave gate and up of a token in one thread.  The
-//                 tokens are the 8 columns, so one read of a weight serves them all.
-//   mid_kernel    8-bit weights only: quantises h per (token, expert) row, which needs the
-//                 row's maximum; with adapters: A2 h.
-//   down_kernel   a CTA owns a few rows of `out` and runs over all routed slots, so the
+//   prep_kernel   where up cannot make it itself: x quantised for 8-bit weights (more than
+//                 8192 values), A13 x of the adapters.
+//   up_kernel     [G; U] and h.  A tile is 8 (gate, up) row pairs of one slot: as the 16 rows
+//                 of an m16n8k16 product they leave gate and up of a token in one thread.
+//                 The tokens are the 8 columns, so one read of a weight serves them all.
+//   mid_kernel    h quantised for 8-bit weights, which needs a row's maximum (small rows are
+//                 left to down); A2 h of the adapters.
+//   down_kernel   a CTA owns a few columns of `out` and runs over all routed slots, so the
 //                 sum over a token's experts stays in its registers: no atomics, no second
-//                 pass, the same order of sums in every run.
+//                 pass over out, the same order of sums in every run.
 //
-// tcgen05 is not used: at n tokens an expert the layer does 2n flops a weight, far below
-// the ridge for the token counts a cached step has, and mma.sync takes the weights from
-// registers in the order they arrive.
+// Each kernel lets the next one start early (programmatic dependent launch): its tables are
+// built and its first weights on their way while the one before it finishes; it waits only
+// for what that one computes.
 //
-// Precision: sums in fp32 (int32 for int8, exact).  h keeps 16 bits of mantissa as the sum
-// of two bf16 values (hi + lo), two products with the same weights, so that the layer
-// rounds once, at its output; 8-bit layers round x and h as their scheme defines.
+// Measured on a B200 (CUDA graph of calls on fresh weights; floor = bytes at the 6457.7 GB/s
+// of a copy):
+//   one token of 8 of 64 slots, H 2048, I 768   int8 14.1 us (floor 5.9), bf16 19.1 (11.7);
+//     what is above the floor is latency: reading ids and map, the first and last bytes of
+//     two streams, h between the kernels
+//   8 tokens, 44 experts, H 4096, I 768, fp8    77.6 us (64.5)
+//   16 tokens, 96 experts, H 2048, I 768, int8  83.5 us (70.4)
+//   2 tokens, 4 experts of 352 MB, bf16         225 us (218): 0.97 of the copy rate
+//
+// tcgen05 is not used: at n tokens an expert the layer does 2n flops a weight.  For the n of
+// a cached step (a few) that is far below what mma.sync feeds (520 Tflop/s measured here in
+// bf16, 80 flops for every byte the memory delivers), and mma.sync takes the weights from
+// registers in the order in which they arrive, without a detour over a swizzled tile.
+//
+// Precision: sums in fp32 (int32 for int8, exact).  h, A13 x and A2 h keep 16 bits of mantissa
+// as the sum of two bf16 values (hi + lo), two products with the same weights, so that the
+// layer rounds to 8 bits once, at its output; 8-bit layers round x and h as their scheme
+// defines.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -96,7 +112,6 @@ struct ExpertsArgs {
 struct Routing {
   int* entries;          // [0] entries, [1] does a token repeat a slot, [2] adapted pairs
   unsigned* bits;        // [kMaxPairs / 32] routed slots
-  int* base;             // [kMaxPairs / 32] entries before a word of `bits`
   short* slot;           // [P] slot of an entry
   short* pair_slot;      // [P] slot of a pair, -1 = none
   unsigned char* mask;   // [P] column tiles of an entry with a pair in them
@@ -107,7 +122,7 @@ struct Routing {
   short* list;           // [P] the pairs with adapters
 };
 
-constexpr int kRoutingFixed = 16 + (kMaxPairs / 32) * 8;
+constexpr int kRoutingFixed = 16 + (kMaxPairs / 32) * 4;
 
 __host__ __device__ inline size_t routing_bytes(int P, int NT, bool lora) {
   return kRoutingFixed + ((size_t)P * (2 + 2 + 1 + 16 * NT + (lora ? 10 : 0)) + 15) / 16 * 16 + 16;
@@ -117,7 +132,6 @@ __device__ __forceinline__ Routing routing_at(unsigned char* base, int P, int NT
   Routing r;
   r.entries = reinterpret_cast<int*>(base);
   r.bits = reinterpret_cast<unsigned*>(base + 16);
-  r.base = reinterpret_cast<int*>(r.bits + kMaxPairs / 32);
   r.col = reinterpret_cast<short*>(base + kRoutingFixed);
   r.slot = r.col + (size_t)P * 8 * NT;
   r.pair_slot = r.slot + P;
