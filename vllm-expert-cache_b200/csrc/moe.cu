@@ -794,10 +794,10 @@ struct UpTiles {
 struct UpTile {
   int e, i0, n;
   __device__ __forceinline__ void at(const UpTiles& t, int i) {
-    e = i / t.per_entry;
+    e = (unsigned)i / (unsigned)t.per_entry;
     const int j = i - e * t.per_entry;
-    i0 = (int)((long long)j * t.I / t.per_entry);
-    n = (int)((long long)(j + 1) * t.I / t.per_entry) - i0;
+    i0 = (unsigned)(j * t.I) / (unsigned)t.per_entry;              // (at most I * I / 8 < 2^31)
+    n = (unsigned)((j + 1) * t.I) / (unsigned)t.per_entry - i0;
   }
 };
 
@@ -1292,8 +1292,8 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
   using Stream = Fifo<KB, kDownChunks[HS] / KB>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
-  const int r0 = (int)((long long)a.H * blockIdx.x / gridDim.x);
-  const int r1 = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x), rows = r1 - r0;
+  const int r0 = (unsigned)a.H * blockIdx.x / gridDim.x;
+  const int r1 = (unsigned)a.H * (blockIdx.x + 1) / gridDim.x, rows = r1 - r0;
   Stream fifo(smem);
   constexpr int kFifo = Stream::kStages * Stream::kStage;
   const Routing rt = routing_at(smem + kFifo, P, NT);
