@@ -464,3 +464,54 @@ def test_experts_h_in_segments(moe, kind, T, k, S, H, I, L, r):
         got = moe.experts(x, w, ids, w13, w2, **args)
         check(got, *moe_ref.experts(x, w, ids, w13, w2, s13, s2))
         assert torch.equal(got, moe.experts(x, w, ids, w13, w2, **args))
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+@pytest.mark.parametrize("T,H,I", [(2, 128, 64), (12, 256, 96), (20, 96, 4096), (32, 128, 64)])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_experts_bad_weights_stay_with_the_tokens_routed_there(moe, kind, T, H, I, bad):
+    """An infinity or a NaN in an expert's weights reaches the tokens that are routed to it
+    and leaves the others' bits alone."""
+    g = gen(T + I)
+    S, k, v = 12, 3, float(bad)
+    w13, w2, s13, s2 = weights_of(g, kind, S, I, H)
+    x = normal(g, T, H)
+    w, ids = routing(g, T, k, S - 1)
+    ids[T // 2, 1] = ids[0, 2] = S - 1              # the bad one, of two tokens
+    hit = [0, T // 2]
+    others = [t for t in range(T) if t not in hit]
+    clean = moe.experts(x, w, ids, w13, w2, w13_scale=s13, w2_scale=s2)
+    where = [lambda: w2[S - 1].view(-1)[::7].fill_(v), lambda: w13[S - 1].view(-1)[::5].fill_(v)]
+    if kind != "bf16":
+        where = [lambda: s2[S - 1].fill_(v), lambda: s13[S - 1, 3].fill_(v)]
+    if kind == "fp8":                               # (e4m3 has a NaN of its own)
+        where.append(lambda: w2[S - 1].view(torch.uint8).view(-1)[::7].fill_(0x7f))
+    for plant in where:
+        plant()
+        got = moe.experts(x, w, ids, w13, w2, w13_scale=s13, w2_scale=s2)
+        assert torch.equal(got[others], clean[others])
+        assert not torch.isfinite(got[hit]).all(1).any()
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+@pytest.mark.parametrize("T,H,I,r", [(2, 128, 64, 8), (12, 256, 96, 16), (20, 96, 4096, 136)])
+@pytest.mark.parametrize("matrix", range(4))
+def test_experts_lora_bad_adapter_stays_with_its_tokens(moe, kind, T, H, I, r, matrix):
+    g = gen(T + r)
+    S, k, L = 6, 3, 3
+    w13, w2, s13, s2 = weights_of(g, kind, S, I, H)
+    lora = adapters_of(g, L, S, r, H, I)
+    x = normal(g, T, H)
+    w, ids = routing(g, T, k, S)
+    adapter = torch.arange(T, dtype=torch.int32, device=DEV) % (L + 1) - 1
+    hit = [t for t in range(T) if t % (L + 1) == 2]                # adapter 1
+    others = [t for t in range(T) if t not in hit]
+
+    def run():
+        return moe.experts_lora(x, w, ids, w13, w2, *lora, adapter, w13_scale=s13, w2_scale=s2)
+
+    clean = run()
+    lora[matrix][1].view(-1)[::11].fill_(float("nan"))
+    got = run()
+    assert torch.equal(got[others], clean[others])
+    assert not hit or not torch.isfinite(got[hit]).all(1).any()

@@ -989,6 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
       for (; cols; cols &= cols - 1) {
         const int t = __ffs(cols) - 1;
         const unsigned rest = cols & (cols - 1);
+        float one[4] = {};
         for (int at = 0; at < lora_bytes; at += KB * 64) {
           const unsigned f = fifo.front();
 #pragma unroll
@@ -1003,19 +1004,19 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
               read_u(t, at + j * 64, v);
             }
             const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              // (a product with zeros in the other column tiles: a branch around it would
-              // index the accumulators at run time and put them into local memory)
-              const bool here = NT == 1 || t >> 3 == nt;
-              chunk_mma_bf16(add[nt], add[nt], wa, zero, here ? v[0] : zero);
-              chunk_mma_bf16(add[nt], add[nt], wa, zero, here ? v[1] : zero);
-              chunk_mma_bf16(add[nt], add[nt], zero, wb, here ? v[2] : zero);
-              chunk_mma_bf16(add[nt], add[nt], zero, wb, here ? v[3] : zero);
-            }
+            chunk_mma_bf16(one, one, wa, zero, v[0]);
+            chunk_mma_bf16(one, one, wa, zero, v[1]);
+            chunk_mma_bf16(one, one, zero, wb, v[2]);
+            chunk_mma_bf16(one, one, zero, wb, v[3]);
           }
           push();
         }
+        // (only the column itself: a row of B13 with an infinity or a NaN is one in them all)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t == nt * 8 + 2 * q + (i & 1)) add[nt][i] = one[i];
       }
     }
     if (!mine) continue;
@@ -1384,6 +1385,7 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
         // an adapted pair: B2's rows with v in its token's column
         const int p = rt.list[u - units.units], t = token_of(a, p);
         const uint4 zero = make_uint4(0, 0, 0, 0);
+        float one[4] = {};
         for (int at = 0; at < lora_bytes; at += KB * 64) {
           const unsigned f = fifo.front();
 #pragma unroll
@@ -1402,15 +1404,16 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
               lo = load_or_zero(a.v_lo + (size_t)p * a.lora.r + pos / 2, in);
             }
             const uint4 wa = load_shared(f + j * 1024), wb = load_shared(f + j * 1024 + 512);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const bool here = NT == 1 || t >> 3 == nt;
-              chunk_mma_bf16(acc[nt], acc[nt], wa, wb, here ? hi : zero);
-              chunk_mma_bf16(acc[nt], acc[nt], wa, wb, here ? lo : zero);
-            }
+            chunk_mma_bf16(one, one, wa, wb, hi);
+            chunk_mma_bf16(one, one, wa, wb, lo);
           }
           push();
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t == nt * 8 + 2 * q + (i & 1)) acc[nt][i] += one[i];
         continue;
       }
       const int e = units.entry(u), end = units.end(u);
@@ -1427,7 +1430,7 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
       }
       // column g's h (its low part at `low` bytes), in shared or in global memory
       const unsigned char* from[NT];
-      bool has[NT];
+      bool has[NT], kept[NT][2];     // column g has a pair; columns 2q, 2q + 1
       const long long low = HS ? stride
                                : reinterpret_cast<const unsigned char*>(a.h_lo) -
                                      reinterpret_cast<const unsigned char*>(a.h_hi);
@@ -1440,8 +1443,10 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
         else
           from[nt] = (WT == kBf16 ? reinterpret_cast<const unsigned char*>(a.h_hi) : a.hq) +
                      (long long)p * row_bytes + b * (KB * 64) + q * 16;
+        const int p0 = col[nt * 8 + 2 * q], p1 = col[nt * 8 + 2 * q + 1];
+        kept[nt][0] = p0 >= 0;
+        kept[nt][1] = p1 >= 0;
         if (WT != kBf16) {
-          const int p0 = col[nt * 8 + 2 * q], p1 = col[nt * 8 + 2 * q + 1];
           if (p0 >= 0) cf[nt][0] = HS ? scale[p0] : __ldcg(a.h_scale + p0);
           if (p1 >= 0) cf[nt][1] = HS ? scale[p1] : __ldcg(a.h_scale + p1);
         }
@@ -1513,6 +1518,8 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
         if (NT > 1 && !(mask >> nt & 1)) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          // (a column without a pair is zeros, but zero times an infinite weight is a NaN)
+          if (!kept[nt][i & 1]) continue;
           const Acc v = whole(sum, nt, i);
           acc[nt][i] += WT == kBf16 ? (float)v : (float)v * (rf[i >> 1] * cf[nt][i & 1]);
         }
