@@ -1647,6 +1647,8 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(const __grid_co
     copy_commit();
   };
   for (int i = 0; i < kRouteStages; ++i) push();
+  // the first CTA's shared memory is there to be written once its threads run
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   if (tid < TT) odd[tid] = some[tid] = 0;
   __syncthreads();
@@ -1674,6 +1676,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(const __grid_co
     }
   }
   __syncthreads();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 
   for (int e = e0 + warp * EX; e < e1; e += kRouteWarps * EX) {
     const bool two = e + 1 < e1;
