@@ -2212,11 +2212,12 @@ int expert_cache_route(const void* x, int T, int ldx, int H, const void* gate_w,
   a.sigmoid = scoring;
   a.renorm = renormalize != 0;
   a.scale = scale;
-  // Tokens a cluster: more of them share a read of the weight once the SMs are filled.
-  // Clusters of 16 CTAs while they all fit the device and there are experts for them (one
+  // Tokens a cluster: as few as keep the clusters to one wave, of which the device holds 15
+  // with 8 CTAs each (32 tokens of 256 experts of 4096: 28.4 us in 16 clusters, 21.5 in 8).
+  // Clusters of 16 CTAs, of which it holds 7, while there are few and experts for them (one
   // token of 128 experts 7.2 -> 6.1 us; 53 tokens of 61 experts 8.2 -> 9.2).  An expert a
   // warp at a time where that is enough for the CTA's share.
-  int tt = T <= 4 ? 1 : T <= 36 ? 2 : 4;
+  int tt = T <= 4 ? 1 : T <= 30 ? 2 : 4;
   while (tt > 1 && route_bytes(tt, H, E) > kSmem - 64) tt /= 2;
   const int cluster = E >= 128 && (T + tt - 1) / tt <= 4 ? 16 : 8;
   return E <= cluster * kRouteWarps ? run_tokens<1>(a, stream, tt, cluster)
