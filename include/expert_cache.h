@@ -183,6 +183,8 @@ EXPERT_CACHE_API int expert_cache_pregate(const void* x, int T, int ldx, int H,
  * out_ids [T*k] int32 and out_weights [T*k] fp32 are in descending order of the picked
  * value.  Ties go to the lower expert id.  NaN and -inf are never picked: where fewer than
  * k experts are left, the id is -1 and the weight 0.
+ * A score of +inf gives its token NaN softmax weights, as the formula does; weights that
+ * sum to 0 are not divided.
  *
  * Returns -1 if:
  *   - T < 0;
@@ -219,6 +221,7 @@ EXPERT_CACHE_API int expert_cache_experts_workspace(int T, int k, int H, int I, 
  * with expert ids, or the composed map of expert_cache_manage_ep with global ids).  A pair
  * whose id or slot is out of range adds nothing; its weight is not read into the result.
  * A token without any pair gets zeros.  The same slot may appear more than once in a token.
+ * An infinity or a NaN, in a token's x or in the weights it is routed to, stays in its row.
  *
  *   x        [T, H] bf16, row stride ldx elements         out  [T, H] bf16, stride ldo
  *   ids      [T, k] int32                                 weights [T, k] fp32

@@ -26,10 +26,10 @@
 //
 // Measured on a B200 (CUDA graph of calls on fresh weights; floor = bytes at the 6457.7 GB/s
 // of a copy):
-//   one token of 8 of 64 slots, H 2048, I 768   int8 14.1 us (floor 5.9), bf16 19.1 (11.7);
+//   one token of 8 of 64 slots, H 2048, I 768   int8 13.5 us (floor 5.9), bf16 18.7 (11.7);
 //     what is above the floor is latency: reading ids and map, the first and last bytes of
 //     two streams, h between the kernels
-//   8 tokens, 44 experts, H 4096, I 768, fp8    77.6 us (64.5)
+//   8 tokens, 44 experts, H 4096, I 768, fp8    76.7 us (64.5)
 //   16 tokens, 96 experts, H 2048, I 768, int8  83.5 us (70.4)
 //   2 tokens, 4 experts of 352 MB, bf16         225 us (218): 0.97 of the copy rate
 //

@@ -14,6 +14,7 @@ the layer's arithmetic on them, for the few tokens of a decode step:
 
 All run on the current stream of the tensors' device, allocate their outputs and workspace
 from torch's caching allocator, read nothing back and can be captured into CUDA graphs.
+They serve only: none has a backward pass, and their results carry no gradient.
 ``ExpertSlotCache.forward`` runs them as one cached step.  They have no counterpart in the
 reference, which leaves the layer to vLLM's kernels (vllm_expert_cache/cache.py:118-163
 ends with the gathered slots).
