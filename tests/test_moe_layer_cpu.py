@@ -267,3 +267,15 @@ def test_forward_refuses_a_step_wider_than_the_slots(monkeypatch):
         cache.forward(x[:2], w[:2], torch.zeros(2, 2, dtype=torch.int32), adapters=(1,) * 5)
     cache.forward(x[:2], w[:2], torch.zeros(2, 2, dtype=torch.int32))
     assert len(calls) == 1 and calls[0][1]["expert_map"] is cache.table
+
+
+@pytest.mark.parametrize("ids,weights", [(torch.uint32, torch.float32), (torch.int16, torch.float32),
+                                         (torch.int32, torch.int32)])
+def test_routing_of_other_types_keeps_the_stock_kernel(monkeypatch, ids, weights):
+    layer = Layer()
+    method = Method(layer)
+    _, calls, _ = armed(layer, method, monkeypatch)
+    method.apply(layer=layer, x=torch.ones(2, H, dtype=torch.bfloat16),
+                 topk_weights=torch.ones(2, 2, dtype=weights),
+                 topk_ids=torch.zeros(2, 2, dtype=ids))
+    assert method.stock == 1 and not calls
