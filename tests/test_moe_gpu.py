@@ -515,3 +515,90 @@ def test_experts_lora_bad_adapter_stays_with_its_tokens(moe, kind, T, H, I, r, m
     got = run()
     assert torch.equal(got[others], clean[others])
     assert not hit or not torch.isfinite(got[hit]).all(1).any()
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+def test_experts_lora_repeated_slots(moe, kind):
+    """A token that names an expert twice, or two experts in one slot: each pair adds its
+    own, and with its own expert's adapter."""
+    g = gen(77)
+    T, k, S, H, I, L, r = 6, 4, 5, 128, 64, 2, 8
+    w13, w2, s13, s2 = weights_of(g, kind, S, I, H)
+    x = normal(g, T, H)
+    w, ids = routing(g, T, k, S)
+    lora = adapters_of(g, L, 2 * S, r, H, I)
+    table = (torch.arange(2 * S, dtype=torch.int32, device=DEV) % S).contiguous()
+    ids[1] = ids[1, 0]
+    ids[2, 1], ids[4, 3] = ids[2, 0] + S, ids[4, 0] + S        # another expert, the same slot
+    adapter = torch.tensor([0, 1, 0, -1, 1, 0], dtype=torch.int32, device=DEV)
+    got = moe.experts_lora(x, w, ids, w13, w2, *lora, adapter, w13_scale=s13, w2_scale=s2,
+                           expert_map=table)
+    check(got, *moe_ref.experts(x, w, ids, w13, w2, s13, s2, table, lora, adapter), kind)
+
+
+def test_layers_on_two_streams_at_once(moe):
+    """Calls in flight on two streams, of kernels that start early and share SMs: each has
+    the bits of a call alone."""
+    g = gen(78)
+    T, k, S, H, I, E = 6, 4, 24, 512, 256, 64
+    work = []
+    for kind in DTYPES:
+        w13, w2, s13, s2 = weights_of(g, kind, S, I, H)
+        lora = adapters_of(g, 2, S, 16, H, I)
+        gate = normal(g, E, H, std=0.1)
+        adapter = torch.arange(T, dtype=torch.int32, device=DEV) % 3 - 1
+        table = (torch.arange(E, dtype=torch.int32, device=DEV) % S).contiguous()
+
+        def layer(x, w13=w13, w2=w2, s13=s13, s2=s2, lora=lora, gate=gate):
+            w, ids = moe.route(x, gate, k)
+            x = moe.experts(x, w, ids, w13, w2, w13_scale=s13, w2_scale=s2, expert_map=table)
+            return moe.experts_lora(x, w, ids, w13, w2, *lora, adapter, w13_scale=s13,
+                                    w2_scale=s2, expert_map=table)
+
+        work.append(layer)
+    xs = [normal(g, T, H) for _ in range(8)]
+    want = [[f(x) for f in work] for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for x in xs * 4:
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append([f(x) for f in work])
+    torch.cuda.synchronize()
+    for mine in got:
+        for i, outs in enumerate(mine):
+            for o, v in zip(outs, want[i % len(xs)]):
+                assert torch.equal(o, v)
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing needs a call outside of a capture first."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from vllm_expert_cache import moe
+g = torch.Generator(device="cuda").manual_seed(1)
+def n(*s):
+    return (torch.randn(s, generator=g, device="cuda") * 0.1).bfloat16()
+x, gate, w13, w2 = n(3, 256), n(128, 256), n(128, 128, 256), n(128, 256, 64)
+lora = n(2, 128, 16, 256), n(2, 128, 128, 8), n(2, 128, 8, 64), n(2, 128, 256, 8)
+c, ad = torch.ones(2, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda") % 2
+def layer():
+    w, ids = moe.route(x, gate, 4)
+    return moe.experts(x, w, ids, w13, w2), moe.experts_lora(x, w, ids, w13, w2, *lora, c, ad)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = layer()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, layer()):
+    assert torch.equal(a, b) and a.abs().max() > 0
+"""
+    root = Path(__file__).resolve().parent.parent / "vllm-expert-cache_b200"
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
