@@ -20,7 +20,6 @@ framework's kernels while it is true.
 
 from __future__ import annotations
 
-import functools
 import sys
 from pathlib import Path
 
@@ -223,9 +222,7 @@ def run(s):
     return _plain_route(s) if s["case"]["kind"] == "route" else _plain_experts(s)
 
 
-@functools.cache
 def _moe():
-    """The framework's module, imported once, as a user's program does."""
     root = str(Path(__file__).resolve().parents[1] / "vllm-expert-cache_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
