@@ -528,7 +528,7 @@ __device__ __forceinline__ float quant_scale(float top) {
 
 template <int WT>
 __device__ __noinline__ unsigned quantise_exactly(float v, float top) {
-  if (top > 1e36f) {             // v * Q must not overflow
+  if (top > 0x1p119f) {          // v * Q must not overflow: 2^119 * 448 < 2^128
     v *= 0x1p-20f;
     top *= 0x1p-20f;
   }
