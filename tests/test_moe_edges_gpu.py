@@ -44,3 +44,23 @@ def test_experts_rows_next_to_the_largest_floats(moe, kind, T, at):
     assert torch.isfinite(want).all() and (want[at].abs() > 1e-6).any()
     off = ((got.double() - want).abs() / bound)[at].max().item()
     assert off <= 1.0, f"{off:.3f} of the bound"
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_infinite_scores(moe, scoring, renormalize):
+    """A score of +inf makes its token's softmax weights NaN; a sigmoid takes it as 1."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(4, 64, generator=g, device=DEV).abs().to(torch.bfloat16)
+    gate = torch.randn(9, 64, generator=g, device=DEV).to(torch.bfloat16)
+    x[0, 0] = x[2, 0] = 0                           # 0 times the infinity: a NaN, never picked
+    gate[5, 0] = float("inf")
+    gate[0:5, 0] = gate[6:, 0] = 0
+    gate[5, 1:] = 0
+    w, ids = moe.route(x, gate, 6, scoring=scoring, renormalize=renormalize)
+    rw, rids = moe_ref.route(x, gate, 6, scoring, renormalize=renormalize)
+    assert torch.equal(ids, rids)
+    torch.testing.assert_close(w.double(), rw, rtol=2.0 ** -23, atol=1e-37, equal_nan=True)
+    for t in (1, 3):
+        assert ids[t, 0] == 5
+        assert w[t].isnan().all() if scoring == "softmax" else torch.isfinite(w[t]).all()

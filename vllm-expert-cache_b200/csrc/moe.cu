@@ -1809,7 +1809,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(const __grid_co
     double total = weight;
 #pragma unroll
     for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-    if (total > 0.0) weight /= total;
+    if (total != 0.0) weight /= total;           // (a NaN, from a score of +inf, is one in all)
   }
   if (lane < a.k) {
     a.weights[(long long)tok * a.k + lane] = mine >= 0 ? (float)(weight * (double)a.scale) : 0.f;
