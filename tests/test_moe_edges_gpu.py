@@ -64,3 +64,27 @@ def test_route_infinite_scores(moe, scoring, renormalize):
     for t in (1, 3):
         assert ids[t, 0] == 5
         assert w[t].isnan().all() if scoring == "softmax" else torch.isfinite(w[t]).all()
+
+
+def test_rows_further_apart_than_32_bits(moe):
+    """x whose rows are 2^32 elements and a row apart: a stride cut to 32 bits is the row
+    itself, and would read the second token from behind the first."""
+    S, H, I, k = 2, 64, 32, 2
+    a = moe_close.inputs("bf16", 2, k, S, H, I, device=DEV)
+    far = 2 ** 32 + H
+    big = torch.empty(far + H, dtype=torch.bfloat16, device=DEV)
+    big[H:2 * H] = 7                                # what a cut stride reads
+    x = big.as_strided((2, H), (far, 1))
+    x.copy_(a["x"])
+    got = moe.experts(x, a["weights"], a["ids"], a["w13"], a["w2"])
+    assert moe_close.worst(got, *moe_close.layer(**a)) <= 1.0
+    gate = a["w13"][0]
+    got, want = moe.route(x, gate, 4), moe.route(a["x"], gate, 4)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_map_of_more_than_32_bits_is_refused(moe):
+    a = moe_close.inputs("bf16", 2, 2, 2, 64, 32, device=DEV)
+    emap = torch.empty(2 ** 32 + 4, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="expert_map"):
+        moe.experts(a["x"], a["weights"], a["ids"], a["w13"], a["w2"], expert_map=emap)

@@ -41,6 +41,7 @@ MAX_SLOTS = 1024        # EXPERT_CACHE_MAX_SLOTS
 MAX_RANK = 256          # EXPERT_CACHE_LORA_MAX_RANK
 MAX_HIDDEN = 16384      # EXPERT_CACHE_PREGATE_MAX_HIDDEN
 MAX_EXPERTS = 2048      # EXPERT_CACHE_PREGATE_MAX_EXPERTS
+MAX_INT = 2 ** 31 - 1   # the C-ABI's int: ctypes cuts what is larger to 32 bits
 
 _BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 # The current stream's handle without building a Stream object (2 us a call).
@@ -56,8 +57,10 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as the kernels read it: bf16 rows of unit inner stride, 16-byte aligned."""
     if x.dtype is not _BF16 or x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"x must be a 2-D bf16 tensor on a GPU, not {_is(x)}")
+    if x.size(0) > MAX_INT:
+        raise ValueError(f"{x.size(0)} rows of x: up to {MAX_INT} are supported")
     row = x.stride(0)
-    if x.stride(1) != 1 or row % 8 or row < x.size(1) or x.data_ptr() % 16:
+    if x.stride(1) != 1 or row % 8 or not x.size(1) <= row <= MAX_INT or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
@@ -202,10 +205,10 @@ def _layer(fn, x, topk_weights, topk_ids, w13, w2, w13_scale, w2_scale, expert_m
     at_map = n_map = 0
     if expert_map is not None:
         n_map = expert_map.numel()
-        if expert_map.dtype is not _I32 or n_map == 0 or expert_map.dim() != 1 \
+        if expert_map.dtype is not _I32 or not 0 < n_map <= MAX_INT or expert_map.dim() != 1 \
                 or not expert_map.is_contiguous() or expert_map.get_device() != index:
-            raise ValueError("expert_map must be a contiguous, non-empty int32 vector beside "
-                             f"x, not {_is(expert_map)}")
+            raise ValueError("expert_map must be a contiguous, non-empty int32 vector of up to "
+                             f"{MAX_INT} entries beside x, not {_is(expert_map)}")
         at_map = expert_map.data_ptr()
     r, more = 0, ()
     if adapters is not None:
