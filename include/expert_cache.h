@@ -193,7 +193,9 @@ EXPERT_CACHE_API int expert_cache_pregate(const void* x, int T, int ldx, int H,
  *   - E <= 0 or E > EXPERT_CACHE_PREGATE_MAX_EXPERTS;
  *   - k outside [1, min(E, EXPERT_CACHE_EXPERTS_MAX_TOPK)];
  *   - scoring outside {0, 1}, or a bias with scoring 0;
- *   - x or gate_w is not 16-byte aligned.
+ *   - x or gate_w is not 16-byte aligned;
+ *   - the tokens need more than 2^31 - 1 CTAs: 8 for every 4 of them (2 or 1 where H or E
+ *     leave no room for more).
  * T == 0 enqueues nothing.
  *
  * Has no counterpart in the reference, whose routing is vLLM's. */

@@ -20,3 +20,14 @@ def test_more_rows_than_32_bits_are_refused():
         w = torch.empty(2, 16, 8, dtype=torch.bfloat16, device="cuda")
         with pytest.raises(ValueError, match="rows of x"):
             moe.experts(x, weights, ids, w, w.view(2, 8, 16)[:, :, :8])
+
+
+@pytest.mark.parametrize("T", [2 ** 30, 2 ** 31 - 4, 2 ** 31 - 1])
+def test_router_refuses_more_tokens_than_a_launch_takes(T):
+    """Before CUDA is touched, and without a sum past the end of int."""
+    import build_lib
+    from vllm_expert_cache import _lib
+    build_lib.build()
+    at = 1 << 20                                    # never dereferenced
+    assert _lib.lib().expert_cache_route(at, T, 8, 8, at, 4, 1, 0, 1, None, 1.0, at, at,
+                                         None) == -1

@@ -2053,7 +2053,7 @@ int run_route(const RouteArgs& a, cudaStream_t stream, int cluster) {
     wide[dev].store(n > 0 ? 1 : 2, std::memory_order_relaxed);
   }
   if (cluster > 8 && wide[dev].load(std::memory_order_relaxed) == 2) cluster = 8;
-  return launch(fn, dim3((a.T + TT - 1) / TT * cluster), kRouteThreads, smem, stream, cluster, a);
+  return launch(fn, dim3((unsigned)(((long long)a.T + TT - 1) / TT * cluster)), kRouteThreads, smem, stream, cluster, a);
 }
 
 template <int EX>
@@ -2092,12 +2092,12 @@ int experts_checked(ExpertsArgs a, int wtype, void* workspace, long workspace_by
   if (!workspace || misaligned(workspace, 256) || workspace_bytes < (long)need) return -1;
   carve(&a, static_cast<unsigned char*>(workspace), per, a.k, a.H, a.I, wtype, r);
   const ExpertsArgs all = a;
-  for (int t = 0; t < T; t += per) {
-    a.T = T - t < per ? T - t : per;
+  for (long long t = 0; t < T; t += per) {       // (T may lie next to the end of int)
+    a.T = T - t < per ? (int)(T - t) : per;
     a.x = all.x + t * all.ldx;
     a.out = all.out + t * all.ldo;
-    a.ids = all.ids + (long long)t * all.k;
-    a.weights = all.weights + (long long)t * all.k;
+    a.ids = all.ids + t * all.k;
+    a.weights = all.weights + t * all.k;
     if (r) a.lora.index = all.lora.index + t;
     a.prepared = wtype != kBf16 && (long long)a.T * a.H > kSelfX;
     const int rc = wtype == kBf16   ? run_type<kBf16>(a, stream)
@@ -2219,7 +2219,9 @@ int expert_cache_route(const void* x, int T, int ldx, int H, const void* gate_w,
   // warp at a time where that is enough for the CTA's share.
   int tt = T <= 4 ? 1 : T <= 30 ? 2 : 4;
   while (tt > 1 && route_bytes(tt, H, E) > kSmem - 64) tt /= 2;
-  const int cluster = E >= 128 && (T + tt - 1) / tt <= 4 ? 16 : 8;
+  const long long groups = ((long long)T + tt - 1) / tt;
+  if (groups * 8 > INT_MAX) return -1;           // CTAs of one launch
+  const int cluster = E >= 128 && groups <= 4 ? 16 : 8;
   return E <= cluster * kRouteWarps ? run_tokens<1>(a, stream, tt, cluster)
                                     : run_tokens<2>(a, stream, tt, cluster);
 }
