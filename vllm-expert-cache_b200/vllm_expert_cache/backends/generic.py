@@ -451,7 +451,7 @@ def arm(layer, method, logger) -> bool:
 
     def own_step(x, topk_weights, topk_ids, shared_experts) -> bool:
         return (own_kernel and shared_experts is None and topk_ids.dim() == 2
-                and topk_ids.size(1) <= moe.MAX_TOPK
+                and topk_ids.size(0) <= moe.STEP_TOKENS and topk_ids.size(1) <= moe.MAX_TOPK
                 and topk_ids.dtype in (torch.int32, torch.int64) and isinstance(x, torch.Tensor)
                 and x.dim() == 2 and x.dtype == torch.bfloat16
                 and x.size(1) == cache.slots["w2_weight"].size(1)
