@@ -313,7 +313,8 @@ def _own_kernel_unusable(layer, method, cache: ExpertSlotCache, cfg) -> str | No
     It computes SwiGLU experts in vLLM's registered weight layout (gate rows, then up rows),
     in bf16 or with 8-bit weights of one scale per output row and activations quantised per
     token, so the stock kernel has to be one that does the same from the same layout, with
-    nothing dispatched to other ranks around it.
+    nothing dispatched to other ranks around it.  (Of 8-bit layers vLLM 0.22 describes fp8 ones
+    so; its dynamic int8 layers have bf16 activations.)
     """
     kernel = method.moe_kernel
     if type(kernel.fused_experts).__name__ != "TritonExperts":

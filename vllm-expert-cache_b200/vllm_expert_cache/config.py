@@ -32,10 +32,12 @@ cache.py:96-97, _lib.py:18, README.md:103-116):
                                   expert_cache_step launch; '0': two launches (manage +
                                   remap, then gather), the form used above 256 slots (new)
   EXPERT_CACHE_MOE        0       '1': a cached step of up to 8 tokens of a layer that the
-                                  library's own kernels can compute (bf16, or int8 / fp8
-                                  W8A8 with dynamic per-token activations; SwiGLU) runs
+                                  library's own kernels can compute (bf16, or fp8 W8A8
+                                  with dynamic per-token activations; SwiGLU) runs
                                   expert_cache_experts on the slots instead of vLLM's
-                                  fused-MoE kernel (new, off by default)
+                                  fused-MoE kernel (new, off by default).  vLLM 0.22 runs
+                                  dynamic int8 layers with bf16 activations: these keep
+                                  its kernel
 
 ``slots_for(E)`` clamps to [1, E]: EXPERT_CACHE_SLOTS=0 means one slot, not "off".
 """
