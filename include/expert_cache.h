@@ -173,8 +173,8 @@ EXPERT_CACHE_API int expert_cache_pregate(const void* x, int T, int ldx, int H,
 /* The router: the k best experts of each token and their weights.
  *
  * The score of an expert is the dot product of x[t, :H] (bf16, row stride ldx elements)
- * with gate_w[e, :H] (bf16, [E, H] row-major), summed in 64 bits, so that the choice does
- * not depend on the order of a sum.
+ * with gate_w[e, :H] (bf16, [E, H] row-major), summed in 64 bits in an order that does not
+ * depend on T: the same token gets the same experts in every call.
  *   scoring 0  softmax over all E experts; the k largest scores are picked
  *   scoring 1  sigmoid of each score; the k largest sigmoid + bias[e] are picked (bias:
  *              fp32 [E] or NULL), the weight is the sigmoid alone
@@ -233,7 +233,8 @@ EXPERT_CACHE_API int expert_cache_experts_workspace(int T, int k, int H, int I, 
  *            bf16).  x and h are then quantised per row: q = round(v * Q / m), scale m / Q,
  *            m = max|v| (at least 1e-10), Q = 127 or 448.
  *
- * Sums are in fp32 (int32 for int8 products); h is not rounded to 16 bits.  The result does
+ * Sums are in fp32 (int32 for int8 products).  bf16 layers hold weights[t, j] * h to 2^-17 of
+ * its value (the sum of two bf16 values); 8-bit layers quantise h from fp32.  The result does
  * not depend on T or on other tokens, up to the order of the sum over a token's experts
  * (ascending slot).  No atomics: the same inputs give the same bits.
  *

@@ -66,6 +66,18 @@ def test_route_infinite_scores(moe, scoring, renormalize):
         assert w[t].isnan().all() if scoring == "softmax" else torch.isfinite(w[t]).all()
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_of_a_token_is_the_same_in_every_batch(moe, scoring):
+    """Bit for bit: a score is summed in one order whatever the batch."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(53, 1000, generator=g, device=DEV).to(torch.bfloat16)
+    gate = (torch.randn(300, 1000, generator=g, device=DEV) * 0.03).to(torch.bfloat16)
+    w, ids = moe.route(x, gate, 8, scoring=scoring)
+    for lo, n in ((0, 1), (52, 1), (7, 3), (20, 5), (4, 30)):
+        part = moe.route(x[lo:lo + n], gate, 8, scoring=scoring)
+        assert torch.equal(part[0], w[lo:lo + n]) and torch.equal(part[1], ids[lo:lo + n])
+
+
 def test_rows_further_apart_than_32_bits(moe):
     """x whose rows are 2^32 elements and a row apart: a stride cut to 32 bits is the row
     itself, and would read the second token from behind the first."""

@@ -29,18 +29,19 @@
 //   one token of 8 of 64 slots, H 2048, I 768   int8 13.5 us (floor 5.9), bf16 18.7 (11.7);
 //     what is above the floor is latency: reading ids and map, the first and last bytes of
 //     two streams, h between the kernels
-//   8 tokens, 44 experts, H 4096, I 768, fp8    76.7 us (64.5)
-//   16 tokens, 96 experts, H 2048, I 768, int8  83.5 us (70.4)
-//   2 tokens, 4 experts of 352 MB, bf16         225 us (218): 0.97 of the copy rate
+//   8 tokens, 44 experts, H 4096, I 768, fp8    76.6 us (64.5)
+//   16 tokens, 96 experts, H 2048, I 768, int8  83.7 us (70.4)
+//   2 tokens, 4 experts of 352 MB, bf16         228 us (218): 0.96 of the copy rate
 //
 // tcgen05 is not used: at n tokens an expert the layer does 2n flops a weight.  For the n of
 // a cached step (a few) that is far below what mma.sync feeds (520 Tflop/s measured here in
 // bf16, 80 flops for every byte the memory delivers), and mma.sync takes the weights from
 // registers in the order in which they arrive, without a detour over a swizzled tile.
 //
-// Precision: sums in fp32 (int32 for int8, exact).  h, A13 x and A2 h keep 16 bits of mantissa
-// as the sum of two bf16 values (hi + lo), two products with the same weights, so that the
-// layer rounds to 8 bits once, at its output; 8-bit layers round x and h as their scheme
+// Precision: sums in fp32 (int32 for int8, exact).  bf16 layers hold weights[t,j] * h, and all
+// layers the adapters' A13 x and A2 h, as the sum of two bf16 values (hi + lo, off by 2^-17 at
+// most where fp32 would be by 2^-24), two products with the same weights, so that the layer
+// rounds to 8 bits once, at its output; 8-bit layers round x and h (from fp32) as their scheme
 // defines.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -796,7 +797,7 @@ struct UpTile {
   __device__ __forceinline__ void at(const UpTiles& t, int i) {
     e = (unsigned)i / (unsigned)t.per_entry;
     const int j = i - e * t.per_entry;
-    i0 = (unsigned)(j * t.I) / (unsigned)t.per_entry;              // (at most I * I / 8 < 2^31)
+    i0 = (unsigned)(j * t.I) / (unsigned)t.per_entry;              // (at most I * I <= 2^30)
     n = (unsigned)((j + 1) * t.I) / (unsigned)t.per_entry - i0;
   }
 };
@@ -806,6 +807,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
   using K = Kind<WT>;
   using Acc = typename K::Acc;
   constexpr int KB = kUpBlock;
+  static_assert(KB == 4, "a block of the staged x is four chunks");
   using Stream = Fifo<KB, kUpStages>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int P = a.T * a.k;
@@ -973,8 +975,7 @@ __global__ void __launch_bounds__(kThreads, 1) up_kernel(const __grid_constant__
         }
       }
       push();      // into the stage just read, whose vectors the products have taken
-      if (KB == 4 || (at & 128)) blk += a.T * 256 - (KB == 2 ? 128 : 0);
-      else blk += 128;
+      blk += a.T * 256;
     }
     // Adapters: one more product for each adapted column, B13's rows with u in that column
     // alone.  Gate and up have different u, so each takes its half of the 16 rows.
@@ -1554,8 +1555,8 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
 // memory, where a warp per token picks.  One launch, bound by latency: reading x and the
 // weight, summing, k dependent choices.
 //
-// Scores are sums in 64 bits of exact products, so which expert is the k-th best does not
-// hang on the order of a sum.  A bf16 becomes a double by moving its bits: shifted by 3 into
+// Scores are sums in 64 bits of exact products, in one order for every call: only experts whose
+// scores agree to some 15 digits could change places with another order.  A bf16 becomes a double by moving its bits: shifted by 3 into
 // a double's high word, its exponent reads as e - 896 (subnormals included).  x is brought
 // back to its own exponent when it is staged, the weights are not: sums are multiplied by
 // 2^896 at the end, which is exact.  (The conversion instruction runs at a quarter of the

@@ -97,9 +97,9 @@ def route(x: torch.Tensor, gate_w: torch.Tensor, k: int, *, scoring: str = "soft
 
     ``scoring`` "softmax" takes the softmax over all experts; "sigmoid" takes each score's
     sigmoid and picks by sigmoid + ``bias`` (fp32 [E], optional).  ``renormalize`` divides a
-    row's weights by their sum; ``scale`` multiplies them.  Scores are summed in 64 bits and
-    ties go to the lower id, so the choice is the same whatever the order of a sum.  NaN
-    scores are never picked; a row with fewer than k others ends in id -1, weight 0.
+    row's weights by their sum; ``scale`` multiplies them.  Scores are summed in 64 bits, in
+    one order whatever the batch, and ties go to the lower id.  NaN scores are never picked; a
+    row with fewer than k others ends in id -1, weight 0.
     """
     mode = SCORING.get(scoring)
     if mode is None:
