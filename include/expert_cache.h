@@ -239,7 +239,8 @@ EXPERT_CACHE_API int expert_cache_experts_workspace(int T, int k, int H, int I, 
  * (ascending slot).  No atomics: the same inputs give the same bits.
  *
  * The weights are read once per 32 tokens (fewer where the tables or 8-bit rows of x do
- * not fit on chip): meant for the steps a cache serves, tokens * k <= S.
+ * not fit on chip): meant for the steps a cache serves, tokens * k <= S, and nearest to the
+ * memory's rate up to 8 tokens.
  *
  * `workspace` (256-byte aligned) is the call's own from its start to its end on `stream`;
  * nothing is kept in it between calls.  out must not overlap an input.

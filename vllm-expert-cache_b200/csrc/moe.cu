@@ -1556,13 +1556,13 @@ __global__ void __launch_bounds__(HS && NT < 4 ? kDownMaxThreads : kThreads, 1)
 // weight, summing, k dependent choices.
 //
 // Scores are sums in 64 bits of exact products, in one order for every call: only experts whose
-// scores agree to some 15 digits could change places with another order.  A bf16 becomes a double by moving its bits: shifted by 3 into
-// a double's high word, its exponent reads as e - 896 (subnormals included).  x is brought
-// back to its own exponent when it is staged, the weights are not: sums are multiplied by
-// 2^896 at the end, which is exact.  (The conversion instruction runs at a quarter of the
-// 64-bit products' rate.)  A sum is done again with plain conversions where the move does not
-// hold: with an infinity or a NaN among its operands, a subnormal in x, or a result so small
-// that products may have underflowed.
+// scores agree to some 15 digits could change places with another order.  A bf16 becomes a
+// double by moving its bits: shifted by 3 into a double's high word, its exponent reads as
+// e - 896 (subnormals included).  x is brought back to its own exponent when it is staged, the
+// weights are not: sums are multiplied by 2^896 at the end, which is exact.  (The conversion
+// instruction runs at a quarter of the 64-bit products' rate.)  A sum is done again with plain
+// conversions where the move does not hold: with an infinity or a NaN among its operands, a
+// subnormal in x, or a result so small that products may have underflowed.
 
 constexpr int kRouteThreads = 512, kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteStages = 8;                  // of a warp, 256 columns of its experts each
@@ -2054,7 +2054,8 @@ int run_route(const RouteArgs& a, cudaStream_t stream, int cluster) {
     wide[dev].store(n > 0 ? 1 : 2, std::memory_order_relaxed);
   }
   if (cluster > 8 && wide[dev].load(std::memory_order_relaxed) == 2) cluster = 8;
-  return launch(fn, dim3((unsigned)(((long long)a.T + TT - 1) / TT * cluster)), kRouteThreads, smem, stream, cluster, a);
+  const long long groups = ((long long)a.T + TT - 1) / TT;
+  return launch(fn, dim3((unsigned)(groups * cluster)), kRouteThreads, smem, stream, cluster, a);
 }
 
 template <int EX>
